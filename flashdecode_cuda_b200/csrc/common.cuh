@@ -23,6 +23,7 @@ constexpr int STATUS_BAD_TOKEN = 1;       // token id outside the embedding tabl
 constexpr int STATUS_BAD_BLOCK = 2;       // block table entry < 0 or >= num_blocks where a token lies
 constexpr int STATUS_BAD_POSITION = 4;    // position beyond the rotation table
 constexpr int STATUS_WAIT_TIMEOUT = 8;    // a bounded mbarrier wait gave up
+constexpr int STATUS_BAD_INDEX = 16;      // a row, block, slot or adapter that does not exist
 
 __device__ __forceinline__ void set_status(int* status, int bit) {
     if (status != nullptr) atomicOr(status, bit);

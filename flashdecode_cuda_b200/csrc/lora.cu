@@ -1,0 +1,207 @@
+// Low-rank adapters of many requests beside a shared projection: out[t] = y[t] + scale B (A x[t]), each token with its adapter's
+// matrices.  This is the form for every type and size; lora_mma.cu has the ones for bfloat16 on the tensor cores.
+//
+// One launch.  A cluster of CTAs takes a tile of up to 16 tokens of one adapter: each CTA multiplies its share of K (A x is a long
+// sum for few values), the partial sums are added over the cluster out of shared memory in the order of the ranks, and each
+// CTA expands its share of the N columns.  A x never leaves the chip and no second launch waits for the first.
+// All sums are 32-bit; one rounding at the end.  The cuts of K depend on the sizes alone, so that no bit of a token's result
+// depends on the other tokens of the step.
+#include <cooperative_groups.h>
+
+#include "lora.cuh"
+
+namespace fd {
+
+namespace cg = cooperative_groups;
+
+constexpr int LR_THREADS = 256, LR_WARPS = LR_THREADS / 32;
+constexpr int LR_ROWS = 16;              // tokens of a tile
+constexpr int LR_CHUNK = 512;            // columns of x in shared memory at once
+constexpr int LR_J = 4;                  // rows of A that a warp multiplies at once: each x out of shared memory is used four times
+
+template <typename T> __device__ __forceinline__ void load4(const T* p, float v[4], bool whole, int n) {
+    if (whole) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p);
+            v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+            v[0] = __low2float(h[0]); v[1] = __high2float(h[0]); v[2] = __low2float(h[1]); v[3] = __high2float(h[1]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? to_float(p[e]) : 0.f;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(LR_THREADS)
+lora_general_kernel(const LoraArgs p) {
+    extern __shared__ __align__(16) float lr_smem[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int Rp = (p.R + 3) & ~3, W = p.S * Rp;                 // a token's A x: S slices of Rp places
+    float* xs = lr_smem;                                         // [LR_ROWS][LR_CHUNK]
+    float* part = xs + LR_ROWS * LR_CHUNK;                       // [LR_ROWS][W] this CTA's sums
+    float* h = part + LR_ROWS * W;                               // [LR_ROWS][W] the cluster's
+    __shared__ int tok[LR_ROWS];
+    __shared__ LoraTile tile_s;
+    if (warp == 0) {
+        const LoraTile f = lora_tile(p, blockIdx.x / C, LR_ROWS);
+        if (lane < LR_ROWS) {
+            int t = lane < f.count ? p.order[f.begin + lane] : -1;
+            if (lane < f.count && (t < 0 || t >= p.T)) { set_status(p.status, STATUS_BAD_INDEX); t = -1; }
+            tok[lane] = t;
+        }
+        if (lane == 0) tile_s = f;
+    }
+    __syncthreads();
+    const LoraTile tile = tile_s;
+    if (tile.adapter == -2) return;                              // the same for the whole cluster
+    // this CTA's columns of the output
+    const int per = (((p.N + 7) / 8 + C - 1) / C) * 8, n0 = rank * per, n1 = min(p.N, n0 + per);
+    const T* y = static_cast<const T*>(p.y);
+    T* out = static_cast<T*>(p.out);
+    if (tile.adapter < 0) {
+        if (static_cast<const void*>(out) == p.y) return;
+        for (int i = 0; i < tile.count; ++i)
+            if (tok[i] >= 0)
+                for (int n = n0 + tid; n < n1; n += LR_THREADS) out[(size_t)tok[i] * p.N + n] = y[(size_t)tok[i] * p.N + n];
+        return;
+    }
+    const int e = tile.adapter, r = min(max(p.ranks[e], 0), p.R);
+    const T* x = static_cast<const T*>(p.x);
+    const T* a = static_cast<const T*>(p.a) + (size_t)e * p.S * p.R * p.K;
+    for (int i = tid; i < LR_ROWS * W; i += LR_THREADS) part[i] = 0.f;
+
+    // --- A x over this CTA's share of K
+    const int kper = (((p.K + 3) / 4 + C - 1) / C) * 4, k0 = rank * kper, k1 = min(p.K, k0 + kper);
+    constexpr unsigned long long unit = 4 * sizeof(T) - 1;       // rows that begin where four values can be loaded at once
+    const bool whole4 = (p.K & 3) == 0 && ((reinterpret_cast<unsigned long long>(p.x) | reinterpret_cast<unsigned long long>(p.a)) & unit) == 0;
+    for (int c0 = k0; c0 < k1; c0 += LR_CHUNK) {
+        const int w = min(LR_CHUNK, k1 - c0), w4 = (w + 3) / 4;
+        __syncthreads();
+        for (int i = tid; i < LR_ROWS * w4; i += LR_THREADS) {
+            const int row = i / w4, c = (i - row * w4) * 4;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            if (tok[row] >= 0) load4(x + (size_t)tok[row] * p.K + c0 + c, v, whole4, w - c);
+            *reinterpret_cast<float4*>(xs + row * LR_CHUNK + c) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        __syncthreads();
+        for (int u0 = warp * LR_J; u0 < p.S * r; u0 += LR_WARPS * LR_J) {
+            float acc[LR_J * LR_ROWS];
+#pragma unroll
+            for (int i = 0; i < LR_J * LR_ROWS; ++i) acc[i] = 0.f;
+            const T* rows[LR_J];
+            int place[LR_J];
+#pragma unroll
+            for (int j = 0; j < LR_J; ++j) {
+                const int u = min(u0 + j, p.S * r - 1), s = u / r;
+                rows[j] = a + (size_t)(s * p.R + (u - s * r)) * p.K + c0;
+                place[j] = u0 + j < p.S * r ? s * Rp + (u - s * r) : -1;
+            }
+            for (int c = lane * 4; c < w; c += 128) {
+                float av[LR_J][4];
+#pragma unroll
+                for (int j = 0; j < LR_J; ++j) load4(rows[j] + c, av[j], whole4, w - c);
+#pragma unroll
+                for (int i = 0; i < LR_ROWS; ++i) {
+                    const float4 xv = *reinterpret_cast<const float4*>(xs + i * LR_CHUNK + c);
+#pragma unroll
+                    for (int j = 0; j < LR_J; ++j)
+                        acc[j * LR_ROWS + i] += av[j][0] * xv.x + av[j][1] * xv.y + av[j][2] * xv.z + av[j][3] * xv.w;
+                }
+            }
+            // 64 sums over the lanes: halves are exchanged, so that after five steps each lane has two of them
+            int first = 0;
+#pragma unroll
+            for (int o = 16, n = LR_J * LR_ROWS / 2; o >= 1; o >>= 1, n >>= 1) {
+                const bool up = (lane & o) != 0;
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const float give = up ? acc[i] : acc[i + n], keep = up ? acc[i + n] : acc[i];
+                    acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+                first += up ? n : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int j = (first + i) / LR_ROWS, row = (first + i) % LR_ROWS;
+                int pl = place[0];
+#pragma unroll
+                for (int q = 1; q < LR_J; ++q) pl = j == q ? place[q] : pl;
+                if (pl >= 0) part[row * W + pl] += acc[i];
+            }
+        }
+    }
+    cluster.sync();
+    for (int i = tid; i < LR_ROWS * W; i += LR_THREADS) {
+        float v = 0.f;
+        for (int c = 0; c < C; ++c) v += *cluster.map_shared_rank(part + i, c);
+        h[i] = v;
+    }
+    cluster.sync();                                              // the others' sums have been read, and h is whole
+
+    // --- B h over this CTA's columns
+    const T* b = static_cast<const T*>(p.b) + (size_t)e * p.N * p.R;
+    const float scale = p.scale[e];
+    const bool vec = (p.R & 3) == 0 && (reinterpret_cast<unsigned long long>(p.b) & unit) == 0;
+    for (int n = n0 + tid; n < n1; n += LR_THREADS) {
+        const int s = p.col_slice != nullptr ? min((int)p.col_slice[n >> 3], p.S - 1) : 0;
+        const T* bn = b + (size_t)n * p.R;
+        const float* hs = h + s * Rp;
+        float acc[LR_ROWS];
+#pragma unroll
+        for (int i = 0; i < LR_ROWS; ++i) acc[i] = 0.f;
+        for (int j = 0; j < r; j += 4) {
+            float bv[4];
+            load4(bn + j, bv, vec, r - j);
+#pragma unroll
+            for (int i = 0; i < LR_ROWS; ++i) {
+                const float4 hv = *reinterpret_cast<const float4*>(hs + i * W + j);
+                acc[i] += bv[0] * hv.x + bv[1] * hv.y + bv[2] * hv.z + bv[3] * hv.w;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < LR_ROWS; ++i)
+            if (i < tile.count && tok[i] >= 0) {
+                const size_t o = (size_t)tok[i] * p.N + n;
+                out[o] = from_float<T>(to_float(y[o]) + scale * acc[i]);
+            }
+    }
+}
+
+// CTAs of a cluster: enough to spread one tile's matrices, by the sizes alone.
+static int lora_cluster(const LoraArgs& p) {
+    const int most = p.K > p.N ? p.K : p.N;
+    return most >= 1024 ? 8 : (most >= 512 ? 4 : (most >= 256 ? 2 : 1));
+}
+
+template <typename T>
+static int launch_general(const LoraArgs& p, cudaStream_t stream) {
+    const int C = lora_cluster(p), W = p.S * ((p.R + 3) & ~3);
+    const size_t smem = sizeof(float) * (LR_ROWS * LR_CHUNK + 2 * (size_t)LR_ROWS * W);
+    const long long tiles = lora_max_tiles(p, LR_ROWS);
+    FD_REQUIRE(tiles * C < (1ll << 31), -2, "lora_add: %d tokens", p.T);
+    const cudaError_t err = cudaFuncSetAttribute(lora_general_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
+    return launch("lora_add", lora_general_kernel<T>, dim3((unsigned)(tiles * C)), dim3(LR_THREADS), smem, stream, dim3(C, 1, 1), p);
+}
+
+}  // namespace fd
+
+using namespace fd;
+
+extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const float* scale, const int* ranks, const int* order,
+                           const int* start, const int* ids, const void* y, void* out, const unsigned char* col_slice, int dtype,
+                           int T, int K, int N, int E, int R, int S, int n_seg, int* status, cudaStream_t stream) {
+    if (T == 0 || N == 0 || n_seg == 0) return 0;
+    FD_REQUIRE(T > 0 && K > 0 && N > 0 && E > 0 && R > 0 && n_seg > 0, -2,
+               "lora_add: %d tokens, %d x %d, %d adapters of rank %d, %d segments", T, K, N, E, R, n_seg);
+    FD_REQUIRE(S >= 1 && S <= 4, -2, "lora_add: %d packed projections; 1 to 4 are taken", S);
+    FD_REQUIRE(R <= 256 && S * R <= 512, -2, "lora_add: rank %d of %d packed projections; up to 256, and 512 in all, are taken", R, S);
+    FD_REQUIRE(S == 1 || (col_slice != nullptr && N % 8 == 0), -2, "lora_add: %d packed projections need col_slice and N a multiple of 8", S);
+    const LoraArgs p{x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status, T, K, N, E, R, S, n_seg};
+    return dtype == 0 ? launch_general<float>(p, stream) : launch_general<__nv_bfloat16>(p, stream);
+}

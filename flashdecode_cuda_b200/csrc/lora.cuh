@@ -1,0 +1,74 @@
+// What the kernels of the low-rank adapters share: their arguments, and the way from a tile's number to its tokens.
+#pragma once
+
+#include "common.cuh"
+
+namespace fd {
+
+// out[t] = y[t] + scale[e] B_e (A_e x[t]), e the adapter of token t.  Tokens come in the order `order`, cut by `start` into segments
+// of one adapter each (`ids`; -1: no adapter, out[t] = y[t]).  a [E][S R][K], b [E][N][R]: a packed product of S projections has an
+// A of its own for each; tile of 8 columns c / 8 belongs to projection col_slice[c / 8] (null: S = 1).  Adapter e uses the first
+// ranks[e] of the R rows and columns.
+struct LoraArgs {
+    const void* x;
+    const void* a;
+    const void* b;
+    const float* scale;
+    const int* ranks;
+    const int* order;
+    const int* start;
+    const int* ids;
+    const void* y;
+    void* out;
+    const unsigned char* col_slice;
+    int* status;
+    int T, K, N, E, R, S, n_seg;
+};
+
+struct LoraTile {
+    int adapter;             // -1: the tokens have none;  -2: there is no such tile
+    int begin, count;        // its tokens are order[begin] .. order[begin + count - 1]
+};
+
+// Tile number `tile` of the segments cut into tiles of `rows` tokens.  Called by one whole warp; every lane gets the answer.
+__device__ __forceinline__ LoraTile lora_tile(const LoraArgs& p, int tile, int rows) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    LoraTile f{-2, 0, 0};
+    for (int base = 0; base < p.n_seg; base += 32) {
+        int lo = 0, n = 0;
+        if (base + lane < p.n_seg) {
+            lo = p.start[base + lane];
+            const int hi = p.start[base + lane + 1];
+            n = hi - lo;
+            if (lo < 0 || n < 0 || hi > p.T) { set_status(p.status, STATUS_BAD_INDEX); n = 0; }
+        }
+        const int tiles = (n + rows - 1) / rows;
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + sum > tile);
+        if (hit != 0u) {
+            const int src = __ffs(hit) - 1;
+            const int skipped = tile - before - __shfl_sync(0xffffffffu, sum - tiles, src);
+            f.begin = __shfl_sync(0xffffffffu, lo, src) + skipped * rows;
+            f.count = min(rows, __shfl_sync(0xffffffffu, n, src) - skipped * rows);
+            f.adapter = p.ids[base + src];
+            if (f.adapter < -1 || f.adapter >= p.E) {
+                set_status(p.status, STATUS_BAD_INDEX);
+                f.adapter = -2;
+            }
+            return f;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return f;
+}
+
+// The most tiles there can be: every segment ends with one that may not be full.
+inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (long long)p.T / rows + p.n_seg; }
+
+}  // namespace fd

@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -27,11 +27,13 @@ STATUS_BAD_TOKEN = 1
 STATUS_BAD_BLOCK = 2
 STATUS_BAD_POSITION = 4
 STATUS_WAIT_TIMEOUT = 8
+STATUS_BAD_INDEX = 16
 _STATUS_TEXT = {
     STATUS_BAD_TOKEN: "a token id lies outside the embedding table",
     STATUS_BAD_BLOCK: "a cached token maps to no allocated block",
     STATUS_BAD_POSITION: "a position lies beyond the rotation table",
     STATUS_WAIT_TIMEOUT: "a bounded wait inside a kernel ran out",
+    STATUS_BAD_INDEX: "a row, block, slot or adapter that does not exist was named",
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -153,6 +155,10 @@ def _declare(L: ctypes.CDLL) -> None:
         "fd_dense_layers": [P, P, I],
         "fd_dense_decode": [P, P, I],
         "fd_sample": [P, I, I, P, P, P, c_ulonglong, P, P, P, P],
+        "fd_beam_select": [P, I, I, P, P, I, I, P, P, P, P, P, P],
+        "fd_copy_blocks": [P, I, LL, I, I, LL, P, P, P, I, P, P],
+        "fd_copy_states": [P, P, I, I, P, P, I, P, P],
+        "fd_lora_add": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, P],
         "fd_copy_h2d_async": [P, P, LL, P],
         "fd_copy_d2h_sync": [P, P, LL, P],
     }
@@ -178,6 +184,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.fd_ssd_chunks_scratch_floats.restype = LL
     L.fd_delta_chunks_scratch_bytes.argtypes = [I, I, I, I]
     L.fd_delta_chunks_scratch_bytes.restype = LL
+    L.fd_beam_select_scratch_bytes.argtypes = [I, I]
+    L.fd_beam_select_scratch_bytes.restype = LL
     L.fd_sample_scratch_words.argtypes = [I, I]
     L.fd_sample_scratch_words.restype = LL
 
@@ -1609,3 +1617,126 @@ def sample(logits: torch.Tensor, out: torch.Tensor, temperature: Optional[torch.
     _check(lib().fd_sample(_ptr(logits), n, V, _ptr(temperature), _ptr(request), _ptr(step),
                            seed & 0xFFFFFFFFFFFFFFFF, _ptr(seed_tensor), _ptr(out), _ptr(scratch) if words else None,
                            _stream()))
+
+
+# ---------------------------------------------------------------------------
+# requests of one batch that differ: several beams each, adapters of their own
+
+BEAM_MAX_ROWS, BEAM_MAX_CANDIDATES = 64, 128
+LORA_MAX_SLICES, LORA_MAX_RANK, LORA_MAX_PACKED = 4, 256, 512
+
+
+def _here(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """All on the device that is current: the launch goes to its stream."""
+    d = first.device
+    if d.type != "cuda":
+        raise KernelError("kernels take CUDA tensors only; there is no CPU path")
+    if d.index != torch.cuda.current_device():
+        raise KernelError(f"the tensors are on {d}, but cuda:{torch.cuda.current_device()} is the current device")
+    for t in others:
+        if t is not None and t.device != d:
+            raise KernelError(f"tensors on {d} and on {t.device} in one call")
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise KernelError(what)
+
+
+def beam_select_scratch_bytes(n: int, V: int) -> int:
+    return int(lib().fd_beam_select_scratch_bytes(n, V))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, row_start: torch.Tensor, out_scores: torch.Tensor,
+                out_rows: torch.Tensor, out_tokens: torch.Tensor, scratch: Optional[torch.Tensor] = None,
+                status: Optional[torch.Tensor] = None) -> None:
+    """The best continuations of every request over its beams and the vocabulary.  Row b of ``logits`` [n, V] (float32) is a
+    beam whose tokens' log-probabilities add up to ``scores[b]``; request r owns the rows ``row_start[r]`` ..
+    ``row_start[r + 1] - 1`` (int32 [R + 1]; at most BEAM_MAX_ROWS of them, none is allowed).  Its k best candidates
+    scores[b] + log_softmax(logits[b])[v], best first, the lower row and then the lower token first where they tie, go to
+    ``out_scores`` (float32), ``out_rows`` and ``out_tokens`` (int32), all [R, k] with k up to BEAM_MAX_CANDIDATES.  A logit of
+    -inf is no candidate; a row whose score or normaliser is no finite number (a NaN or +inf among its logits, nothing but -inf) has
+    none.  Places that no candidate fills: -inf, -1, -1.  ``scratch``: uint8 of ``beam_select_scratch_bytes(n, V)`` that the call may
+    use; when omitted it is allocated."""
+    _need(logits.dim() == 2 and logits.dtype == torch.float32 and scores.dtype == torch.float32, "beam_select: logits [n, V] and scores are float32")
+    n, V = logits.shape
+    R, k = out_scores.shape
+    _need(scores.shape == (n,), f"beam_select: {n} rows of logits, scores {tuple(scores.shape)}")
+    _need(row_start.dtype == torch.int32 and row_start.shape == (R + 1,), f"beam_select: row_start is int32 [{R + 1}]")
+    _need(out_rows.shape == (R, k) and out_tokens.shape == (R, k) and out_scores.dtype == torch.float32
+          and out_rows.dtype == out_tokens.dtype == torch.int32, "beam_select: outputs are float32, int32 and int32, all [R, k]")
+    _here(logits, scores, row_start, out_scores, out_rows, out_tokens, scratch, status)
+    need = lib().fd_beam_select_scratch_bytes(n, V)
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    _need(scratch.dtype == torch.uint8 and scratch.numel() >= need and scratch.data_ptr() % 8 == 0,
+          f"beam_select: scratch is uint8, {need} of them, 8-byte aligned")
+    _check(lib().fd_beam_select(_ptr(logits), n, V, _ptr(scores), _ptr(row_start), R, k, _ptr(out_scores), _ptr(out_rows),
+                                _ptr(out_tokens), _ptr(scratch), _ptr(status), _stream()))
+
+
+def copy_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, count: torch.Tensor,
+                status: Optional[torch.Tensor] = None) -> None:
+    """pool[p, dst[i], :, :count[i]] = pool[p, src[i], :, :count[i]] for every plane p and copy i: the first ``count[i]`` tokens of a
+    cache block.  ``pool`` [planes, blocks, heads, block_size, ...] of any type; ``src``, ``dst``, ``count`` int32 [n].  No block may
+    be named twice in ``dst``, or in both ``src`` and ``dst``.  A block or count outside the pool is skipped and reported."""
+    _need(pool.dim() >= 4, "copy_blocks: the pool is [planes, blocks, heads, block_size, ...]")
+    planes, blocks, heads, size = pool.shape[:4]
+    n = src.numel()
+    _need(src.dtype == dst.dtype == count.dtype == torch.int32 and dst.numel() == n == count.numel(), f"copy_blocks: src, dst and count are int32 [{n}]")
+    _here(pool, src, dst, count, status)
+    if pool.numel() == 0:
+        return
+    row = pool.numel() // (planes * blocks * heads * size) * pool.element_size()
+    _check(lib().fd_copy_blocks(_ptr(pool), planes, blocks, heads, size, row, _ptr(src), _ptr(dst), _ptr(count), n, _ptr(status),
+                                _stream()))
+
+
+def copy_states(states: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, status: Optional[torch.Tensor] = None) -> None:
+    """state[dst[i]] = state[src[i]] for every tensor [slots, ...] of ``states`` and copy i.  ``src``, ``dst`` int32 [n]; no slot may be
+    named twice in ``dst``, or in both.  A slot that does not exist is skipped and reported."""
+    n = src.numel()
+    _need(src.dtype == dst.dtype == torch.int32 and dst.numel() == n, f"copy_states: src and dst are int32 [{n}]")
+    if not states:
+        return
+    slots = states[0].shape[0]
+    _here(src, dst, status, *states)
+    if slots == 0:
+        return
+    for t in states:
+        _need(t.shape[0] == slots, f"copy_states: states of {slots} and of {t.shape[0]} slots")
+    m = len(states)
+    at, size = (c_void_p * m)(*map(_ptr, states)), (c_longlong * m)(*[t.nbytes // slots for t in states])
+    _check(lib().fd_copy_states(at, size, m, slots, _ptr(src), _ptr(dst), n, _ptr(status), _stream()))
+
+
+def lora_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, ranks: torch.Tensor, order: torch.Tensor,
+             start: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None,
+             col_slice: Optional[torch.Tensor] = None, slices: int = 1, status: Optional[torch.Tensor] = None) -> None:
+    """out[t] = y[t] + scale[e] * b[e] (a[e] x[t]), e the adapter of token t: the low-rank terms of many requests at once, beside the
+    shared projection ``y`` [T, N] of ``x`` [T, K].  ``out`` may be ``y`` (and is when it is not given).
+
+    The tokens' adapters: ``order`` (int32 [T]) has every token once, sorted by adapter; the tokens order[start[i]:start[i + 1]] use
+    the adapter ``ids[i]`` (-1: none, out[t] = y[t]); ``start`` int32 [segments + 1], ``ids`` int32 [segments].  Segments may be empty;
+    tokens behind the last one are left as they were.
+
+    The adapters: ``a`` [E, slices * R, K], ``b`` [E, N, R] of x's type, ``scale`` float32 [E], ``ranks`` int32 [E]: adapter e uses the
+    first ranks[e] of the R rows of a and columns of b, and b is zero behind them.  A packed product of several projections (q, k and
+    v; gate and up) has ``slices`` of them: rows s * R .. of a belong to slice s, and a tile of 8 columns to slice
+    ``col_slice[tile]`` (uint8 [N / 8]).  A x is kept in 32 bits (as two bfloat16 numbers where tensor cores multiply it); one
+    rounding.  An adapter, segment or token that does not exist is skipped and reported."""
+    out = y if out is None else out
+    T, Kd = x.shape
+    E, N, R = b.shape
+    _need(x.dtype == a.dtype == b.dtype == y.dtype == out.dtype, "lora_add: x, a, b, y and out are of one type")
+    _need(a.shape == (E, slices * R, Kd), f"lora_add: a is [{E}, {slices * R}, {Kd}], not {tuple(a.shape)}")
+    _need(y.shape == (T, N) and out.shape == (T, N), f"lora_add: y and out are [{T}, {N}]")
+    _need(scale.dtype == torch.float32 and scale.shape == (E,) and ranks.dtype == torch.int32 and ranks.shape == (E,),
+          f"lora_add: scale is float32 [{E}], ranks int32 [{E}]")
+    n_seg = ids.numel()
+    _need(order.dtype == start.dtype == ids.dtype == torch.int32 and order.shape == (T,) and start.shape == (n_seg + 1,),
+          f"lora_add: order, start and ids are int32 [{T}], [{n_seg + 1}], [{n_seg}]")
+    _need(col_slice is None or (col_slice.dtype == torch.uint8 and col_slice.numel() * 8 == N), "lora_add: col_slice is uint8 [N / 8]")
+    _here(x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status)
+    _check(lib().fd_lora_add(_ptr(x), _ptr(a), _ptr(b), _ptr(scale), _ptr(ranks), _ptr(order), _ptr(start), _ptr(ids), _ptr(y),
+                             _ptr(out), _ptr(col_slice), _dt(x.dtype), T, Kd, N, E, R, slices, n_seg, _ptr(status), _stream()))
