@@ -40,12 +40,26 @@ def cmd_generate(args) -> int:
     prompts = _prompts(args)
     stop = [int(t) for t in args.stop_ids.split(",")] if args.stop_ids else \
         (engine.config.stop_token_ids() if args.model else [])
-    max_batch = args.max_batch or min(len(prompts), 64)
+    adapter = None
+    if args.adapter:
+        adapter = "adapter"
+        engine.add_adapter(adapter, args.adapter)
+    max_batch = args.max_batch or (max(args.beams, min(len(prompts) * args.beams, 64)) if args.beams else min(len(prompts), 64))
     longest = args.max_context or max(len(p) for p in prompts) + args.max_new_tokens
     cache = engine.new_paged_cache(max_batch, longest, args.block_size)
     t0 = time.time()
+    if args.beams:
+        found = engine.beam_search(prompts, args.max_new_tokens, cache, num_beams=args.beams, length_penalty=args.length_penalty,
+                                   stop_token_ids=stop, max_batch=max_batch, adapter=adapter)
+        dt = time.time() - t0
+        for r in found:
+            h = r.hypotheses[0]
+            print(json.dumps({"request": r.request_id, "tokens": h.tokens, "finish_reason": h.finish_reason, "score": h.score}))
+        n = sum(len(r.tokens) for r in found)
+        print(f"{n} tokens in {dt:.3f} s ({n / dt:.1f} tok/s of the best hypotheses, prompts included in the time)", file=sys.stderr)
+        return 0
     results = engine.generate(prompts, args.max_new_tokens, cache, temperature=args.temperature,
-                              seed=args.sample_seed, stop_token_ids=stop, max_batch=max_batch)
+                              seed=args.sample_seed, stop_token_ids=stop, max_batch=max_batch, adapter=adapter)
     dt = time.time() - t0
     n = sum(len(r.tokens) for r in results)
     for r in results:
@@ -81,6 +95,9 @@ def main(argv=None) -> int:
     g.add_argument("--block-size", type=int, default=64, help="tokens per cache block")
     g.add_argument("--max-batch", type=int, default=0, help="sequences that run together (default: all, up to 64)")
     g.add_argument("--max-context", type=int, default=0, help="longest sequence the cache is sized for")
+    g.add_argument("--beams", type=int, default=0, help="beam search with so many beams per prompt (default: sampling)")
+    g.add_argument("--length-penalty", type=float, default=1.0, help="beam search: scores are divided by length to this power")
+    g.add_argument("--adapter", help="folder of a low-rank adapter that all prompts use")
     g.add_argument("--device", default="cuda")
     g.set_defaults(fn=cmd_generate)
 

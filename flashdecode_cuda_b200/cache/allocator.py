@@ -2,8 +2,9 @@
 
 The block allocator of davidjoyme/flashdecode-cuda (engine/paged_cache.py:85-119)
 is a LIFO list whose ``free`` builds a set of the whole free list to catch a
-double free; here a per-id flag does that check in O(1).  The same class hands
-out cache blocks and sequence slots.
+double free; here a count of holders per id does that check in O(1).  The same class hands
+out cache blocks and sequence slots.  An id may have several holders (a cache block of beams that
+share a beginning): ``share`` adds one, ``free`` takes one away, and the last one's goes back to the pool.
 """
 
 from __future__ import annotations
@@ -23,7 +24,7 @@ class IdAllocator:
         self.what = what
         # reversed so the first ids handed out are 0, 1, 2, ...
         self._free: List[int] = list(range(count - 1, -1, -1))
-        self._in_use = bytearray(count)
+        self._holders: List[int] = [0] * count
 
     @property
     def num_free(self) -> int:
@@ -34,7 +35,10 @@ class IdAllocator:
         return self.count - len(self._free)
 
     def in_use(self, i: int) -> bool:
-        return 0 <= i < self.count and bool(self._in_use[i])
+        return 0 <= i < self.count and self._holders[i] > 0
+
+    def holders(self, i: int) -> int:
+        return self._holders[i]
 
     def allocate(self, n: int = 1) -> List[int]:
         if n < 0:
@@ -43,8 +47,17 @@ class IdAllocator:
             raise PoolExhausted(f"{self.what} pool exhausted: asked for {n}, {len(self._free)} free of {self.count}")
         out = [self._free.pop() for _ in range(n)]
         for i in out:
-            self._in_use[i] = 1
+            self._holders[i] = 1
         return out
+
+    def share(self, ids: Iterable[int]) -> None:
+        """One more holder for every id."""
+        ids = list(ids)
+        for i in ids:
+            if not self.in_use(i):
+                raise ValueError(f"{self.what} {i} is not in use")
+        for i in ids:
+            self._holders[i] += 1
 
     def free(self, ids: Iterable[int]) -> None:
         ids = list(ids)
@@ -52,9 +65,10 @@ class IdAllocator:
         for i in ids:        # check everything before changing anything
             if not (0 <= i < self.count):
                 raise ValueError(f"{self.what} {i} is outside the pool of {self.count}")
-            if not self._in_use[i] or i in seen:
+            if not self._holders[i] or i in seen:
                 raise ValueError(f"double free of {self.what} {i}")
             seen.add(i)
         for i in ids:
-            self._in_use[i] = 0
-            self._free.append(i)
+            self._holders[i] -= 1
+            if self._holders[i] == 0:
+                self._free.append(i)

@@ -18,6 +18,8 @@ What is different:
   values).  Each group has its own pool, allocator and block table; a window
   group gives blocks back as they fall behind the window, a chunk group those
   that lie wholly before the chunk of the next query;
+* sequences that go on as several beams share the blocks that are full (a block counts its holders); ``fork`` and
+  ``reorder`` copy what they cannot share, for all layers in one launch per pool;
 * beside the paged storage there is per-sequence state of fixed size, indexed
   by slot, for mixers that carry a recurrent state instead of keys.
 
@@ -34,6 +36,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from .. import kernels as K
 from .allocator import IdAllocator, PoolExhausted
 
 FREE, ACTIVE = 0, 1
@@ -91,6 +94,7 @@ class StateSpec:
 class SlotRecord:
     state: int = FREE
     length: int = 0
+    adapter: int = -1                # the low-rank adapter of the sequence's tokens (-1: none)
     blocks: List[List[int]] = field(default_factory=list)      # per group: block id per table column (-1: none)
 
 
@@ -201,15 +205,20 @@ class PagedCache:
         self.lengths_version = 0        # grows whenever a slot's sequence or its length changes (admit, release, advance)
 
     # ------------------------------------------------------------------ slots
-    def admit(self) -> int:
-        """Take a free slot for a new sequence of length 0; its state is zeroed."""
-        (slot,) = self.slot_alloc.allocate(1)
-        rec = self.slots[slot]
-        rec.state, rec.length = ACTIVE, 0
-        self.lengths_version += 1
-        rec.blocks = [[] for _ in self.groups]
+    def admit(self, adapter: int = -1) -> int:
+        """Take a free slot for a new sequence of length 0; its state is zeroed.  ``adapter``: the number of the low-rank
+        adapter that its tokens use (``engine.adapters``)."""
+        slot = self._take_slot(adapter)
         for st in self.states.values():
             st[slot].zero_()
+        return slot
+
+    def _take_slot(self, adapter: int = -1) -> int:
+        (slot,) = self.slot_alloc.allocate(1)
+        rec = self.slots[slot]
+        rec.state, rec.length, rec.adapter = ACTIVE, 0, adapter
+        self.lengths_version += 1
+        rec.blocks = [[] for _ in self.groups]
         return slot
 
     def release(self, slot: int) -> None:
@@ -222,9 +231,141 @@ class PagedCache:
             for col, b in enumerate(blocks):
                 if b >= 0:
                     g.set_entry(slot, col, -1)
-        rec.state, rec.length, rec.blocks = FREE, 0, []
+        rec.state, rec.length, rec.adapter, rec.blocks = FREE, 0, -1, []
         self.lengths_version += 1
         self.slot_alloc.free([slot])
+
+    # ------------------------------------------------------------------ beams
+    def fork(self, pairs: Sequence[Tuple[int, int]]) -> None:
+        """For every (source, destination): the destination's sequence ends, and its slot goes on as a copy of the source's.
+        Blocks that are full are shared; the last, partly filled one and the state are copied.  No slot may be a destination
+        twice, or a source and a destination.  Nothing changes if a group lacks the blocks for it."""
+        if not pairs:
+            return
+        srcs, dsts = [s for s, _ in pairs], [d for _, d in pairs]
+        for slot in srcs + dsts:
+            self._record(slot)
+        if len(set(dsts)) != len(dsts) or set(dsts) & set(srcs):
+            raise ValueError(f"a slot is a destination twice, or a source and a destination: {list(pairs)}")
+        full = [self.slots[s].length // self.block_size for s in srcs]
+        rest = [self.slots[s].length % self.block_size for s in srcs]
+        for gi, g in enumerate(self.groups):
+            change: Dict[int, int] = {}
+            for d in dsts:
+                for b in self.slots[d].blocks[gi]:
+                    if b >= 0:
+                        change[b] = change.get(b, 0) - 1
+            for s, n in zip(srcs, full):
+                for b in self.slots[s].blocks[gi][:n]:
+                    if b >= 0:
+                        change[b] = change.get(b, 0) + 1
+            freed = sum(1 for b, c in change.items() if g.alloc.holders(b) + c == 0)
+            need = sum(1 for r in rest if r)
+            if need > g.alloc.num_free + freed:
+                raise PoolExhausted(f"paged cache exhausted: group {gi} needs {need} blocks for the beams' last tokens, "
+                                    f"{g.alloc.num_free + freed} free of {g.num_blocks}")
+        copies: List[List[Tuple[int, int, int]]] = []
+        for gi, g in enumerate(self.groups):
+            lists = []
+            for s, n in zip(srcs, full):
+                shared = self.slots[s].blocks[gi][:n]
+                g.alloc.share([b for b in shared if b >= 0])
+                lists.append(shared)
+            for d in dsts:
+                g.alloc.free([b for b in self.slots[d].blocks[gi] if b >= 0])
+            todo = []
+            for s, d, n, r, new in zip(srcs, dsts, full, rest, lists):
+                if r:
+                    (block,) = g.alloc.allocate(1)
+                    todo.append((self.slots[s].blocks[gi][n], block, r))
+                    new = new + [block]
+                old = self.slots[d].blocks[gi]
+                for c in range(max(len(old), len(new))):
+                    b = new[c] if c < len(new) else -1
+                    if (old[c] if c < len(old) else -1) != b:
+                        g.set_entry(d, c, b)
+                self.slots[d].blocks[gi] = new
+            copies.append(todo)
+        for s, d in pairs:
+            self.slots[d].length, self.slots[d].adapter = self.slots[s].length, self.slots[s].adapter
+        self.lengths_version += 1
+        self._copy(srcs, dsts, copies)
+
+    def _copy(self, srcs: List[int], dsts: List[int], copies: List[List[Tuple[int, int, int]]]) -> None:
+        """What a fork moves on the device: partly filled blocks (source, destination, tokens) per group, and states."""
+        columns = [list(c) for todo in copies if todo for c in zip(*todo)]
+        if self.states:
+            columns += [srcs, dsts]
+        if not columns:
+            return
+        if self.device.type != "cuda":
+            for g, todo in zip(self.groups, copies):
+                for s, d, n in todo:
+                    for pool in ((g.keys,) if g.values is g.keys else (g.keys, g.values)):
+                        pool[:, d, :, :n] = pool[:, s, :, :n]
+            for st in self.states.values():
+                st[dsts] = st[srcs]
+            return
+        flat = torch.tensor([i for c in columns for i in c], dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        at = 0
+
+        def take(n):
+            nonlocal at
+            at += n
+            return flat[at - n:at]
+        for g, todo in zip(self.groups, copies):
+            if not todo:
+                continue
+            src, dst, count = take(len(todo)), take(len(todo)), take(len(todo))
+            if g.pool is not None:
+                K.copy_blocks(g.pool.view(-1, *g.pool.shape[2:]), src, dst, count)
+            else:
+                for pool in ((g.keys,) if g.values is g.keys else (g.keys, g.values)):
+                    K.copy_blocks(pool, src, dst, count)
+        if self.states:
+            K.copy_states(list(self.states.values()), take(len(srcs)), take(len(srcs)))
+
+    def reorder(self, beams: Sequence[Tuple[Sequence[int], Sequence[int]]]) -> List[List[int]]:
+        """For every (slots of a request's beams, parents): the request goes on with one beam for each parent, a copy of the
+        sequence in that slot (one of its slots; any number of times).  Returns, per request, the slots of its beams in the order of
+        ``parents``.  A parent's first child stays where it is, the others take the slots of sequences without a child, then
+        free ones; slots that are left over are released.  Nothing changes if the slots or blocks do not suffice."""
+        taken: set = set()
+        for slots, parents in beams:
+            if len(set(slots)) != len(slots) or taken & set(slots) or not set(parents) <= set(slots):
+                raise ValueError(f"parents {list(parents)} of the beams in the slots {list(slots)}: every slot belongs to one request, "
+                                 f"once, and a parent is one of its request's slots")
+            taken |= set(slots)
+            for s in slots:
+                self._record(s)
+        out, pairs, new, spare = [], [], [], []
+        try:
+            for slots, parents in beams:
+                unused = [s for s in slots if s not in set(parents)]
+                unused.reverse()
+                placed, row = set(), []
+                for p in parents:
+                    if p not in placed:
+                        placed.add(p)
+                        row.append(p)
+                        continue
+                    if unused:
+                        d = unused.pop()
+                    else:
+                        d = self._take_slot()
+                        new.append(d)
+                    pairs.append((p, d))
+                    row.append(d)
+                out.append(row)
+                spare += unused
+            self.fork(pairs)
+        except PoolExhausted:
+            for d in new:
+                self.release(d)
+            raise
+        for s in spare:
+            self.release(s)
+        return out
 
     def _record(self, slot: int) -> SlotRecord:
         if not (0 <= slot < self.max_slots) or self.slots[slot].state != ACTIVE:
@@ -233,6 +374,10 @@ class PagedCache:
 
     def length(self, slot: int) -> int:
         return self._record(slot).length
+
+    def adapter(self, slot: int) -> int:
+        """The number of the low-rank adapter that the sequence's tokens use; -1: none."""
+        return self._record(slot).adapter
 
     def active_slots(self) -> List[int]:
         return [i for i, r in enumerate(self.slots) if r.state == ACTIVE]
@@ -356,20 +501,26 @@ class PagedCache:
     def check_invariants(self) -> None:
         """No block lost, held twice or free while held; slots likewise."""
         for gi, g in enumerate(self.groups):
-            held: Dict[int, int] = {}
+            held: Dict[int, int] = {}            # block -> its holders among the slots
             for si, rec in enumerate(self.slots):
                 if rec.state != ACTIVE:
                     if rec.blocks:
                         raise AssertionError(f"free slot {si} still lists blocks")
                     continue
-                for b in rec.blocks[gi]:
+                listed = [b for b in rec.blocks[gi] if b >= 0]
+                if len(set(listed)) != len(listed):
+                    raise AssertionError(f"group {gi}: slot {si} lists a block twice")
+                for c, b in enumerate(rec.blocks[gi]):
                     if b < 0:
                         continue
-                    if b in held:
-                        raise AssertionError(f"group {gi}: block {b} held by slots {held[b]} and {si}")
                     if not g.alloc.in_use(b):
                         raise AssertionError(f"group {gi}: block {b} of slot {si} is on the free list")
-                    held[b] = si
+                    if g.alloc.holders(b) > 1 and c >= rec.length // self.block_size:
+                        raise AssertionError(f"group {gi}: slot {si} would write to block {b}, which it shares")
+                    held[b] = held.get(b, 0) + 1
+            for b, n in held.items():
+                if g.alloc.holders(b) != n:
+                    raise AssertionError(f"group {gi}: block {b} counts {g.alloc.holders(b)} holders, {n} slots hold it")
             if len(held) != g.alloc.num_used:
                 raise AssertionError(f"group {gi}: {g.alloc.num_used} blocks marked used, {len(held)} held by slots")
             if g.alloc.num_free + g.alloc.num_used != g.num_blocks:

@@ -71,6 +71,7 @@ lora_general_kernel(const LoraArgs p) {
         return;
     }
     const int e = tile.adapter, r = min(max(p.ranks[e], 0), p.R);
+    if (r == 0 && static_cast<const void*>(out) == p.y) return;   // an adapter that leaves this projection alone
     const T* x = static_cast<const T*>(p.x);
     const T* a = static_cast<const T*>(p.a) + (size_t)e * p.S * p.R * p.K;
     for (int i = tid; i < LR_ROWS * W; i += LR_THREADS) part[i] = 0.f;

@@ -21,7 +21,10 @@ from .. import kernels as K
 from ..cache.paged import DEFAULT_BLOCK_SIZE, PagedCache
 from ..config import load_config
 from ..sampling.sampler import Sampler
+from ..weights import adapters as A
 from ..weights import loader as W
+from .adapters import Adapters
+from .beam import BeamBackend, BeamLoop, BeamRequest, BeamResult
 from .decode import GraphDecoder
 from .generate import Backend, GenerationLoop, Request, Result
 from .model import Model
@@ -38,7 +41,7 @@ def as_dtype(dtype) -> torch.dtype:
         raise ValueError(f"dtype must be one of {sorted(_DTYPES)}, got {dtype!r}") from None
 
 
-class Engine(Backend):
+class Engine(Backend, BeamBackend):
     """A bound model with a sampler; the object ``load`` returns."""
 
     def __init__(self, model: Model):
@@ -73,8 +76,8 @@ class Engine(Backend):
         bs = self.cache.block_size
         return -(-n_tokens // bs) * bs
 
-    def admit(self) -> int:
-        return self.cache.admit()
+    def admit(self, adapter: int = -1) -> int:
+        return self.cache.admit(adapter)
 
     def release(self, slot: int) -> None:
         self.cache.release(slot)
@@ -90,6 +93,26 @@ class Engine(Backend):
         toks = self.sampler.sample(logits, temps, rids, steps, self.seed)
         return toks.tolist()
 
+    # -- Backend of the beam search ------------------------------------------
+    beam_capacity = capacity
+
+    def beam_tokens_held(self, request: BeamRequest) -> int:
+        # every beam may differ from the prompt's last, partly filled block on
+        bs, p = self.cache.block_size, len(request.prompt)
+        return p // bs * bs + request.num_beams * self.tokens_held(p % bs + request.max_new_tokens)
+
+    def reorder(self, beams):
+        return self.cache.reorder(beams)
+
+    def select(self, slots, tokens, scores, row_start, k):
+        if self.use_graphs and all(len(t) == 1 for t in tokens):
+            dec = self._decoder()
+            dec.run(slots, [t[0] for t in tokens])
+            logits = dec.last_logits(len(slots))
+        else:
+            logits = self.model.step(self.cache, slots, tokens, "last")
+        return self.sampler.select_beams(logits, scores, row_start, k)
+
     def _decoder(self) -> GraphDecoder:
         if self._graph_decoder is None or self._graph_decoder.cache is not self.cache:
             self._graph_decoder = GraphDecoder(self.model, self.cache)
@@ -103,21 +126,64 @@ class Engine(Backend):
             raise ValueError("the decoder belongs to another model")
         self._graph_decoder = decoder
 
+    # -- adapters -------------------------------------------------------------
+    def enable_adapters(self, max_adapters: int = 8, max_rank: int = 16) -> Adapters:
+        """Room for low-rank adapters beside the model's products, allocated now (at most once).  ``add_adapter`` does this with
+        these sizes, or the first adapter's rank if that is larger, where it has not been done."""
+        if self.model.adapters is not None:
+            raise RuntimeError("the model has room for adapters already")
+        return Adapters(self.model, max_adapters, max_rank)
+
+    def add_adapter(self, name: str, source, scale: Optional[float] = None) -> int:
+        """Add a low-rank adapter, or replace the one called ``name``: a folder (``adapter_config.json`` +
+        ``adapter_model.safetensors``) or its tensors by name, ``<module>.lora_A.weight`` [r, in] and ``<module>.lora_B.weight``
+        [out, r] with ``scale`` (alpha / r).  Requests choose it by its name (``generate(..., adapter=...)``)."""
+        if isinstance(source, dict):
+            if scale is None:
+                raise ValueError("an adapter given as tensors needs its scale (alpha / rank)")
+            pairs = A.pair_up(source)
+        else:
+            pairs, of_file = A.read_adapter(source)
+            scale = of_file if scale is None else scale
+        if self.model.adapters is None:
+            self.enable_adapters(max_rank=max(16, max(a.shape[0] for a, _ in pairs.values())))
+        return self.model.adapters.put(name, pairs, float(scale))
+
+    def remove_adapter(self, name: str) -> None:
+        if self.model.adapters is None:
+            raise KeyError(f"there is no adapter {name!r}")
+        index = self.model.adapters.index(name)
+        if any(c is not None and any(c.adapter(s) == index for s in c.active_slots()) for c in (self.cache, self._own_cache)):
+            raise RuntimeError(f"adapter {name!r} is in use by a live sequence")
+        self.model.adapters.remove(name)
+
+    def _adapter_numbers(self, adapter, n: int) -> List[int]:
+        names = list(adapter) if isinstance(adapter, (list, tuple)) else [adapter] * n
+        if len(names) != n:
+            raise ValueError(f"{len(names)} adapters for {n} prompts")
+        if all(name is None for name in names):
+            return [-1] * n
+        if self.model.adapters is None:
+            raise KeyError("there are no adapters: add_adapter() comes first")
+        return [self.model.adapters.index(name) for name in names]
+
     # -- generation ---------------------------------------------------------
-    def _requests(self, input_ids, max_new_tokens, temperature, stop_token_ids) -> List[Request]:
+    @staticmethod
+    def _prompts(input_ids) -> List[List[int]]:
         if isinstance(input_ids, torch.Tensor):
             prompts = input_ids.tolist()
-            if input_ids.dim() == 1:
-                prompts = [prompts]
-        else:
-            prompts = [list(map(int, p)) for p in input_ids]
+            return [prompts] if input_ids.dim() == 1 else prompts
+        return [list(map(int, p)) for p in input_ids]
+
+    def _requests(self, input_ids, max_new_tokens, temperature, stop_token_ids, adapter=None) -> List[Request]:
+        prompts = self._prompts(input_ids)
         if stop_token_ids is None:
             stop_token_ids = ()
         n = len(prompts)
         mx = max_new_tokens if isinstance(max_new_tokens, (list, tuple)) else [max_new_tokens] * n
         tp = temperature if isinstance(temperature, (list, tuple)) else [temperature] * n
-        return [Request(p, int(m), float(t), tuple(int(s) for s in stop_token_ids), i)
-                for i, (p, m, t) in enumerate(zip(prompts, mx, tp))]
+        return [Request(p, int(m), float(t), tuple(int(s) for s in stop_token_ids), i, e)
+                for i, (p, m, t, e) in enumerate(zip(prompts, mx, tp, self._adapter_numbers(adapter, n)))]
 
     def _ensure_cache(self, requests: Sequence[Request], cache, max_batch, block_size) -> int:
         max_batch = max_batch or min(len(requests), 64)
@@ -136,15 +202,16 @@ class Engine(Backend):
 
     def generate(self, input_ids, max_new_tokens, cache: Optional[PagedCache] = None, *,
                  temperature=0.0, seed: int = 0, stop_token_ids: Optional[Sequence[int]] = None,
-                 max_batch: Optional[int] = None, block_size: int = DEFAULT_BLOCK_SIZE):
+                 max_batch: Optional[int] = None, block_size: int = DEFAULT_BLOCK_SIZE, adapter=None):
         """Generate up to ``max_new_tokens`` tokens for every prompt.
 
         ``input_ids``: a [B, S] tensor (the reference's form; returns a
         [B, max_new_tokens] int64 tensor, positions after an early stop filled
         with -1) or a list of token lists of unequal lengths (returns a list of
         ``Result``).  ``temperature`` 0 is greedy.  More prompts than
-        ``max_batch`` run as several batches on the same cache."""
-        requests = self._requests(input_ids, max_new_tokens, temperature, stop_token_ids)
+        ``max_batch`` run as several batches on the same cache.  ``adapter``: the name of a low-rank adapter
+        (``add_adapter``), or one name (or None) per prompt."""
+        requests = self._requests(input_ids, max_new_tokens, temperature, stop_token_ids, adapter)
         max_batch = self._ensure_cache(requests, cache, max_batch, block_size)
         self.seed = seed
         results = GenerationLoop(self, max_batch).run(requests)
@@ -158,13 +225,40 @@ class Engine(Backend):
 
     def stream(self, input_ids, max_new_tokens, cache: Optional[PagedCache] = None, *, temperature=0.0,
                seed: int = 0, stop_token_ids: Optional[Sequence[int]] = None, max_batch: Optional[int] = None,
-               block_size: int = DEFAULT_BLOCK_SIZE) -> Iterator[List[Tuple[int, int, Optional[str]]]]:
+               block_size: int = DEFAULT_BLOCK_SIZE, adapter=None) -> Iterator[List[Tuple[int, int, Optional[str]]]]:
         """Like ``generate`` but yields, step by step, the new token of every
         live sequence as host integers: (prompt index, token, finish reason)."""
-        requests = self._requests(input_ids, max_new_tokens, temperature, stop_token_ids)
+        requests = self._requests(input_ids, max_new_tokens, temperature, stop_token_ids, adapter)
         max_batch = self._ensure_cache(requests, cache, max_batch, block_size)
         self.seed = seed
         return GenerationLoop(self, max_batch).events(requests)
+
+    def beam_search(self, input_ids, max_new_tokens, cache: Optional[PagedCache] = None, *, num_beams: int = 4,
+                    length_penalty: float = 1.0, early_stopping: bool = False, num_return: int = 1,
+                    stop_token_ids: Optional[Sequence[int]] = None, max_batch: Optional[int] = None,
+                    block_size: int = DEFAULT_BLOCK_SIZE, adapter=None) -> List[BeamResult]:
+        """The ``num_return`` best of the hypotheses that beam search over ``num_beams`` beams finds for every prompt
+        (``engine.beam`` has its rules), up to ``max_new_tokens`` tokens long.  ``num_beams`` and ``max_new_tokens``: a number, or one
+        per prompt.  ``max_batch``: beams that run together (more prompts run as several batches); ``adapter`` as for
+        ``generate``."""
+        prompts = self._prompts(input_ids)
+        n = len(prompts)
+        mx = list(max_new_tokens) if isinstance(max_new_tokens, (list, tuple)) else [max_new_tokens] * n
+        nb = list(num_beams) if isinstance(num_beams, (list, tuple)) else [num_beams] * n
+        if len(mx) != n or len(nb) != n:
+            raise ValueError(f"{n} prompts, {len(mx)} lengths, {len(nb)} numbers of beams")
+        if not 1 <= num_return <= min(nb, default=1):
+            raise ValueError(f"num_return must lie in 1..num_beams, got {num_return}")
+        stop = tuple(int(s) for s in stop_token_ids or ())
+        requests = [BeamRequest(p, int(m), int(b), float(length_penalty), stop, bool(early_stopping), e, i)
+                    for i, (p, m, b, e) in enumerate(zip(prompts, mx, nb, self._adapter_numbers(adapter, n)))]
+        if not requests:
+            return []
+        max_batch = self._ensure_cache(requests, cache, max_batch or max(max(nb), min(sum(nb), 64)), block_size)
+        results = BeamLoop(self, max_batch).run(requests)
+        for r in results:
+            del r.hypotheses[num_return:]
+        return results
 
     def step(self, cache, slots, tokens, want="last"):
         return self.model.step(cache, slots, tokens, want)

@@ -74,7 +74,7 @@ class GraphDecoder:
         self._ahead: Optional[Tuple] = None
 
     # ------------------------------------------------------------------
-    def _key(self, n: int, longest: int, greedy: bool, seed: int) -> Tuple:
+    def _key(self, n: int, longest: int, greedy: bool, seed: int, adapted: bool = False) -> Tuple:
         # powers of two: a sequence that grows from 1,000 to 4,000 tokens passes three bounds, not four, and a process
         # that captures fewer graphs stays clear of the slower replay that set in after the fourth capture (the same
         # graph 1.25 or 1.33 ms a step; which one changed with captures and large allocations, nothing else)
@@ -82,7 +82,8 @@ class GraphDecoder:
         while bound < longest:
             bound *= 2
         bound = min(bound, self.cache.max_len)
-        return (bucket_of(n), bound, greedy, 0)       # the seed lives in device memory: one graph serves every seed
+        # the seed lives in device memory: one graph serves every seed
+        return (bucket_of(n), bound, greedy, 0, self.model.adapters.made) if adapted else (bucket_of(n), bound, greedy, 0)
 
     def _prepare(self, g: _Graph, key: Tuple, slots: Sequence[int], tokens: Sequence[int]) -> StepContext:
         B, bound = key[0], key[1]
@@ -108,6 +109,8 @@ class GraphDecoder:
         ahead, self._ahead = self._ahead, None
         if ahead is None or ahead[0] is not g or ahead[1] != tuple(slots) or ahead[2] != self.cache.lengths_version:
             self._fill_lengths(g, B, slots)     # else: written while the GPU ran the step before, and still true
+        if g.ctx.lora is not None:              # behind the wanted rows (all B of them)
+            h[8 * B:] = self.model.token_adapters(self.cache, slots, [1] * n, B, g.ctx.lora.ids.numel())
         self.model._staging.upload(h, g.meta)
 
     def _fill_lengths(self, g: _Graph, B: int, slots: Sequence[int]) -> None:
@@ -175,7 +178,8 @@ class GraphDecoder:
         cache.reserve([(s, 1) for s in slots])
         cache.sync()
         longest = max(cache.length(s) for s in slots) + 1
-        key = self._key(n, longest, greedy, seed)
+        adapted = self.model.adapters is not None and any(cache.adapter(s) >= 0 for s in slots)
+        key = self._key(n, longest, greedy, seed, adapted)
         device_fed = tokens is None
         if device_fed:
             if self.last is None or self.last_n != n:

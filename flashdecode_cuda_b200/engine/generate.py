@@ -26,6 +26,7 @@ class Request:
     temperature: float = 0.0
     stop_token_ids: Tuple[int, ...] = ()
     request_id: int = 0
+    adapter: int = -1                # the low-rank adapter that the request's tokens use (-1: none)
 
     def __post_init__(self):
         if len(self.prompt) == 0:
@@ -52,7 +53,8 @@ class Backend:
         """Cache tokens a sequence of ``n_tokens`` occupies (rounded to blocks)."""
         raise NotImplementedError
 
-    def admit(self) -> int:
+    def admit(self, adapter: int = -1) -> int:
+        """A slot for a new sequence; ``adapter`` is given only for requests that use one."""
         raise NotImplementedError
 
     def release(self, slot: int) -> None:
@@ -97,7 +99,8 @@ class GenerationLoop:
             n = plan_batch([r for _, r in waiting], self.max_batch, slots_cap, tokens_cap,
                            self.backend.tokens_held)
             batch, waiting = waiting[:n], waiting[n:]
-            live = [(idx, req, self.backend.admit()) for idx, req in batch]
+            live = [(idx, req, self.backend.admit(req.adapter) if req.adapter >= 0 else self.backend.admit())
+                    for idx, req in batch]
             produced = {idx: 0 for idx, _, _ in live}
             feed = [list(req.prompt) for _, req, _ in live]
             try:

@@ -22,6 +22,7 @@ import torch
 from .. import kernels as K
 from ..cache.paged import DEFAULT_BLOCK_SIZE, KVGroupSpec, PagedCache, StateSpec
 from ..parts.base import KVRequest, LayerCache, Runtime
+from ..parts.lowrank import TokenAdapters
 from ..registry import architecture, part_class
 from ..weights import loader as W
 from .blueprint import ModelBlueprint, PartSpec
@@ -89,6 +90,7 @@ class StepContext:
     # the part that runs now (``Part.first_weights`` of what follows), or None; a part may have its last kernel ask
     # L2 for their beginning
     upcoming: Optional[torch.Tensor] = None
+    lora: Optional[TokenAdapters] = None     # the tokens' low-rank adapters; None: no sequence of the step uses one
 
 
 class _Staging:
@@ -157,6 +159,7 @@ class Model:
         self.trace: Optional[Dict[str, torch.Tensor]] = None    # set to {} to record per-layer activations
         self.last_meta_host: Optional[np.ndarray] = None        # the index array of the last prepared step
         self.bound = False
+        self.adapters = None             # ``engine.adapters.Adapters`` once there are any
         # prompt steps of dense models are launched from native code; None: every step goes through the parts
         self.native: Optional[DensePrompts] = None
 
@@ -374,6 +377,9 @@ class Model:
             np.concatenate([flat.astype(np.int32), np.zeros(pad_rows, np.int32)]), tok_row, tok_pos,
             np.asarray(list(slots) + [-1] * pad_rows, dtype=np.int32), starts, counts_p, ctx_p,
             np.asarray(wanted, dtype=np.int32)])
+        n_seg = self.adapter_segments(cache, slots, N)
+        if n_seg:
+            host = np.concatenate([host, self.token_adapters(cache, slots, counts, T, n_seg)])
         ws = ws or self.ws
         meta = ws.get("step_meta", (host.size,), torch.int32)
         self.last_meta_host = host
@@ -388,10 +394,35 @@ class Model:
         tok, trow, tpos = take(T), take(T), take(T)
         rslot, rstart, rlen, rctx = take(N), take(N), take(N), take(N)
         wrows = take(len(wanted)) if wanted else None
+        lora = TokenAdapters(take(T), take(n_seg + 1), take(n_seg)) if n_seg else None
         longest = max(l + c for l, c in zip(ctx_len, counts))
         return StepContext(self.rt, ws, cache, T, N, tok, trow, tpos, rslot, rstart, rlen, rctx, wrows,
                            len(wanted), int(max(counts)), int(kv_len_bound or longest),
-                           list(slots), counts, ctx_len)
+                           list(slots), counts, ctx_len, lora=lora)
+
+    def adapter_segments(self, cache: PagedCache, slots: Sequence[int], n_rows: int) -> int:
+        """How many segments of tokens by adapter a step of ``n_rows`` rows has room for; 0 where no sequence uses an adapter."""
+        if self.adapters is None or not any(cache.adapter(s) >= 0 for s in slots):
+            return 0
+        return min(n_rows, self.adapters.capacity)
+
+    def token_adapters(self, cache: PagedCache, slots: Sequence[int], counts: Sequence[int], T: int, n_seg: int) -> np.ndarray:
+        """The step's tokens in the order of their adapters, where each adapter's begin, and the adapters: T, n_seg + 1 and n_seg
+        numbers.  Tokens without an adapter (and padding) stand behind the last segment; segments that are not needed are empty."""
+        who = np.full(T, np.iinfo(np.int32).max, dtype=np.int32)
+        used = [cache.adapter(s) for s in slots]
+        real = np.repeat(np.asarray(used, dtype=np.int32), counts)
+        who[:len(real)] = np.where(real < 0, who[:len(real)], real)
+        order = np.argsort(who, kind="stable").astype(np.int32)
+        ids = np.unique(np.asarray([e for e in used if e >= 0], dtype=np.int32))
+        bounds = np.searchsorted(who[order], ids, side="left")
+        end = int((who != np.iinfo(np.int32).max).sum())
+        out = np.full(T + 2 * n_seg + 1, end, dtype=np.int32)
+        out[:T] = order
+        out[T:T + len(ids)] = bounds
+        out[T + n_seg + 1:] = -1
+        out[T + n_seg + 1:T + n_seg + 1 + len(ids)] = ids
+        return out
 
     def forward(self, ctx: StepContext) -> Optional[torch.Tensor]:
         """Run the parts over a prepared step.  Returns logits [n_want, V]

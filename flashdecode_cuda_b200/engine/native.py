@@ -8,8 +8,8 @@ nothing between the layers - the same launches are made by ``fd_dense_layers``
 (up to 128 tokens: the whole step in one call) or, layer by layer, by
 ``fd_dense_mixer`` and ``fd_dense_gate_up`` around the library products of the
 output and down projections.  A decode step of up to 24 sequences is one kernel
-for all layers (``fd_dense_decode``) where it takes the sizes.  Everything else, and every step that this module
-does not take, goes through the parts' ``forward``.
+for all layers (``fd_dense_decode``) where it takes the sizes.  Everything else, every step that this module
+does not take, and steps with low-rank adapters go through the parts' ``forward``.
 
 A part whose ``forward`` was wrapped or replaced, on the object or on its class,
 is called: such a model's steps go through the parts.
@@ -162,7 +162,7 @@ class DensePrompts:
     def takes(self, model, ctx) -> bool:
         """Whether the parts would run this step on the kernels that the native calls launch."""
         T = ctx.T
-        if linear.PROMPT_GEMM != "auto" or ctx.max_q_len < 2 or T <= linear.GEMV_MAX_ROWS:
+        if linear.PROMPT_GEMM != "auto" or ctx.max_q_len < 2 or T <= linear.GEMV_MAX_ROWS or getattr(ctx, "lora", None) is not None:
             return False
         if not self._current(model):
             return False
@@ -175,6 +175,8 @@ class DensePrompts:
         """Whether the step is one token each of so few sequences that one kernel runs all of its layers
         (``csrc/dense_decode.cu``); every layer has to write the keys that it reads."""
         T = ctx.T
+        if getattr(ctx, "lora", None) is not None:
+            return False
         if ctx.max_q_len != 1 or T > (DECODE_MAX_ROWS if linear.PROMPT_GEMM == "auto" else linear.GEMV_MAX_ROWS) or T != ctx.n_rows:
             return False
         if not self._current(model) or not self.all_write:

@@ -11,6 +11,7 @@ from .. import kernels as K
 from ..registry import register_part
 from ..weights.spec import TensorSpec
 from .base import KVRequest, LayerCache, Mixer, Runtime
+from .lowrank import AdaptedProduct
 from .linear import GEMV_MAX_ROWS, UPCOMING_BYTES, fused_prompt_gemm, matmul, stream_gemm
 
 
@@ -159,6 +160,12 @@ class GQAAttention(Mixer):
             n += self.b_qkv.numel() * self.b_qkv.element_size()
         return n
 
+    def adapted_products(self) -> List[AdaptedProduct]:
+        p, d = self.prefix, self.d
+        return [AdaptedProduct("qkv", [f"{p}.{x}_proj" for x in "qkv"], [self.n_q * d, self.n_kv * d, self.n_kv * d], self.hidden_size,
+                               self._paired_order() if self.paired else None),
+                AdaptedProduct("o", [f"{p}.o_proj"], [self.hidden_size], self.n_q * d)]
+
     # --- a step ----------------------------------------------------------
     def first_weights(self) -> Optional[torch.Tensor]:
         return self.w_qkv
@@ -169,7 +176,10 @@ class GQAAttention(Mixer):
         q = ws.get("q_rot", (T, self.n_q * d), x.dtype)
         rope = self.position
         splits = 0
-        if self.paired and x.dtype == torch.bfloat16 and T <= GEMV_MAX_ROWS:
+        lora = self.lora if getattr(ctx, "lora", None) is not None else None
+        # (an adapter's term comes between the product and the rotation: such a step takes them one by one)
+        fuses = self.paired and x.dtype == torch.bfloat16 and lora is None
+        if fuses and T <= GEMV_MAX_ROWS:
             splits = K.gemv_splits(T, self.w_qkv.shape[0], self.hidden_size, 4 * self.rt.sm_count)
         if splits >= 1:
             # decode: projection, bias, rotation and cache append in one kernel
@@ -177,18 +187,20 @@ class GQAAttention(Mixer):
             K.gemv_qkv_rope(x, self.w_qkv, self.b_qkv, q, rope.cos, rope.sin, ctx.tok_row, ctx.tok_pos, ctx.row_slot,
                             lc.k_pool, lc.v_pool, lc.group.table, self.n_q, self.n_kv, d, lc.writes, self.rt.status,
                             splits, prefetch=self.w_o if self.w_o.numel() * 2 <= PREFETCH_BYTES else None)
-        elif self.paired and x.dtype == torch.bfloat16 and stream_gemm(T, self.w_qkv.shape[0], self.hidden_size):
+        elif fuses and stream_gemm(T, self.w_qkv.shape[0], self.hidden_size):
             # larger decode batches and short prompts: the same fusion in the streaming tcgen05 kernel
             K.gemm_stream_qkv_rope(x, self.w_qkv, self.b_qkv, q, rope.cos, rope.sin, ctx.tok_row, ctx.tok_pos,
                                    ctx.row_slot, lc.k_pool, lc.v_pool, lc.group.table, self.n_q, self.n_kv, d,
                                    lc.writes, self.rt.status)
-        elif self.paired and x.dtype == torch.bfloat16 and fused_prompt_gemm(T, self.w_qkv.shape[0], self.hidden_size):
+        elif fuses and fused_prompt_gemm(T, self.w_qkv.shape[0], self.hidden_size):
             # prompts: the same fusion on the tcgen05 tensor cores
             K.gemm_tc_qkv_rope(x, self.w_qkv, self.b_qkv, q, rope.cos, rope.sin, ctx.tok_row, ctx.tok_pos, ctx.row_slot,
                                lc.k_pool, lc.v_pool, lc.group.table, self.n_q, self.n_kv, d, lc.writes, self.rt.status)
         else:
             qkv = ws.get("qkv", (T, (self.n_q + 2 * self.n_kv) * d), x.dtype)
             matmul(x, self.w_qkv, self.b_qkv, qkv, status=self.rt.status)
+            if lora is not None:
+                lora["qkv"].add(x, qkv, ctx.lora)
             K.rope_append(qkv, q, rope.cos, rope.sin, ctx.tok_row, ctx.tok_pos, ctx.row_slot, lc.k_pool, lc.v_pool,
                           lc.group.table, self.n_q, self.n_kv, d, lc.writes, self.rt.status, paired=self.paired)
         attn = ws.get("attn", (T, self.n_q * d), x.dtype)
@@ -217,4 +229,7 @@ class GQAAttention(Mixer):
                          self.rt.status, prefetch=ahead, prefetch_bytes=UPCOMING_BYTES, chunk=self.chunk or 0,
                          **cut)
         out = ws.get("mixer_out", (T, self.hidden_size), x.dtype)
-        return matmul(attn, self.w_o, None, out, target_ctas=4 * self.rt.sm_count, status=self.rt.status)
+        out = matmul(attn, self.w_o, None, out, target_ctas=4 * self.rt.sm_count, status=self.rt.status)
+        if lora is not None:
+            lora["o"].add(attn, out, ctx.lora)
+        return out

@@ -113,6 +113,13 @@ class Part:
     # otherwise decides on the host: its steps cannot be replayed from a CUDA graph.
     graph_safe = True
 
+    # The low-rank adapters of the part's products by ``AdaptedProduct.name`` (``engine.adapters`` sets it); None: it has none
+    lora = None
+
+    def adapted_products(self) -> list:
+        """The products (``parts.lowrank.AdaptedProduct``) that the part can add low-rank adapters to, once it is bound."""
+        return []
+
     def tensor_specs(self) -> List[TensorSpec]:
         return []
 

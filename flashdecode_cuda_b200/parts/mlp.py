@@ -11,6 +11,7 @@ from ..registry import register_part
 from ..weights.spec import TensorSpec
 from .base import FeedForward, Runtime
 from .linear import GEMV_MAX_ROWS, MAX_PARTS, fused_prompt_gemm, matmul, stream_gemm
+from .lowrank import AdaptedProduct
 
 
 @register_part("feed_forward", "swiglu")
@@ -48,6 +49,12 @@ class SwiGLU(FeedForward):
     def weight_bytes(self) -> int:
         return (self.w_gate_up.numel() + self.w_down.numel()) * self.w_down.element_size()
 
+    def adapted_products(self) -> List[AdaptedProduct]:
+        p, H, I = self.prefix, self.hidden_size, self.inter
+        order = torch.arange(2 * I).view(2, I // 8, 8).transpose(0, 1).reshape(-1) if self.tiled else None
+        return [AdaptedProduct("gate_up", [f"{p}.gate_proj", f"{p}.up_proj"], [I, I], H, order),
+                AdaptedProduct("down", [f"{p}.down_proj"], [H], I)]
+
     def first_weights(self) -> Optional[torch.Tensor]:
         return self.w_gate_up
 
@@ -56,23 +63,30 @@ class SwiGLU(FeedForward):
         projection may come back as float32 [parts, T, H] instead."""
         T, ws = ctx.T, ctx.ws
         act = ws.get("ffn_act", (T, self.inter), x.dtype)
-        if (self.tiled and x.dtype == torch.bfloat16 and T <= GEMV_MAX_ROWS
+        lora = self.lora if getattr(ctx, "lora", None) is not None else None
+        fuses = self.tiled and x.dtype == torch.bfloat16 and lora is None       # (an adapter's term comes before the activation)
+        if (fuses and T <= GEMV_MAX_ROWS
                 and K.gemv_splits(T, 2 * self.inter, self.hidden_size, 1, allow_split=False) == 1):
             K.gemv(x, self.w_gate_up, None, act, K.GEMV_GATED)          # product and silu(gate) * up in one kernel
-        elif self.tiled and x.dtype == torch.bfloat16 and stream_gemm(T, 2 * self.inter, self.hidden_size):
+        elif fuses and stream_gemm(T, 2 * self.inter, self.hidden_size):
             K.gemm_stream(x, self.w_gate_up, None, act, gated=True, status=self.rt.status)      # 17 to 128 rows: the same fusion
-        elif self.tiled and x.dtype == torch.bfloat16 and fused_prompt_gemm(T, 2 * self.inter, self.hidden_size):
+        elif fuses and fused_prompt_gemm(T, 2 * self.inter, self.hidden_size):
             K.gemm_tc(x, self.w_gate_up, None, act, gated=True, status=self.rt.status)     # prompts: tcgen05, same fusion
         else:
             gu = ws.get("gate_up", (T, 2 * self.inter), x.dtype)
             matmul(x, self.w_gate_up, None, gu, status=self.rt.status)
+            if lora is not None:
+                lora["gate_up"].add(x, gu, ctx.lora)
             K.silu_mul(gu, act, tiled=self.tiled)
         out = ws.get("ffn_out", (T, self.hidden_size), x.dtype)
         parts = None
-        if parts_ok and T <= GEMV_MAX_ROWS:
+        if parts_ok and T <= GEMV_MAX_ROWS and lora is None:
             parts = ws.get("ffn_out_parts", (MAX_PARTS, T, self.hidden_size), torch.float32)
-        return matmul(act, self.w_down, None, out, target_ctas=4 * self.rt.sm_count, parts=parts, status=self.rt.status,
-                      upcoming=ctx.upcoming)
+        out = matmul(act, self.w_down, None, out, target_ctas=4 * self.rt.sm_count, parts=parts, status=self.rt.status,
+                     upcoming=ctx.upcoming)
+        if lora is not None:
+            lora["down"].add(act, out, ctx.lora)
+        return out
 
 
 @register_part("feed_forward", "gated_mlp")

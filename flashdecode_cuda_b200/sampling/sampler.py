@@ -10,7 +10,7 @@ depend on which other requests share its batch or on its row in it.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -56,3 +56,22 @@ class Sampler:
         stp = torch.from_numpy(np.asarray(steps, dtype=np.int32)).to(self.device)
         K.sample(logits, out, temp, req, stp, seed)
         return out
+
+    def select_beams(self, logits: torch.Tensor, scores: Sequence[float], row_start: Sequence[int], k: int
+                     ) -> Tuple[List[List[float]], List[List[int]], List[List[int]]]:
+        """The k best continuations of every request over its beams (rows ``row_start[r]`` .. ``row_start[r + 1] - 1`` of
+        ``logits``, whose sums of log-probabilities are ``scores``) and the vocabulary: scores, rows and tokens, best first, as host
+        numbers (-inf, -1, -1 behind the last).  One small copy to the device and one back."""
+        n, R = logits.shape[0], len(row_start) - 1
+        if len(scores) != n:
+            raise ValueError(f"{n} rows of logits, {len(scores)} scores")
+        if any(not 0 <= a <= b <= n or b - a > K.BEAM_MAX_ROWS for a, b in zip(row_start[:-1], row_start[1:])):
+            raise ValueError(f"row_start {list(row_start)}: ranges of up to {K.BEAM_MAX_ROWS} of the {n} rows")
+        host = np.empty(n + R + 1, dtype=np.int32)
+        host[:n] = np.asarray(scores, dtype=np.float32).view(np.int32)
+        host[n:] = row_start
+        dev = torch.from_numpy(host).to(self.device)
+        out = torch.empty(3, R, k, dtype=torch.int32, device=self.device)
+        K.beam_select(logits, dev[:n].view(torch.float32), dev[n:], out[0].view(torch.float32), out[1], out[2])
+        back = out.cpu()
+        return back[0].view(torch.float32).tolist(), back[1].tolist(), back[2].tolist()
