@@ -194,6 +194,8 @@ static int launch_general(const LoraArgs& p, cudaStream_t stream) {
 
 using namespace fd;
 
+extern "C" int fd_sm_count();
+
 extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const float* scale, const int* ranks, const int* order,
                            const int* start, const int* ids, const void* y, void* out, const unsigned char* col_slice, int dtype,
                            int T, int K, int N, int E, int R, int S, int n_seg, int* status, cudaStream_t stream) {
@@ -204,5 +206,6 @@ extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const fl
     FD_REQUIRE(R <= 256 && S * R <= 512, -2, "lora_add: rank %d of %d packed projections; up to 256, and 512 in all, are taken", R, S);
     FD_REQUIRE(S == 1 || (col_slice != nullptr && N % 8 == 0), -2, "lora_add: %d packed projections need col_slice and N a multiple of 8", S);
     const LoraArgs p{x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status, T, K, N, E, R, S, n_seg};
-    return dtype == 0 ? launch_general<float>(p, stream) : launch_general<__nv_bfloat16>(p, stream);
+    if (dtype == 0) return launch_general<float>(p, stream);
+    return lora_mma_takes(p) ? lora_rows(p, fd_sm_count(), stream) : launch_general<__nv_bfloat16>(p, stream);
 }

@@ -71,4 +71,8 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& p, int tile, int r
 // The most tiles there can be: every segment ends with one that may not be full.
 inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (long long)p.T / rows + p.n_seg; }
 
+// The kernels on the tensor cores (lora_mma.cu): whether they take the sizes, and the launch.
+bool lora_mma_takes(const LoraArgs& p);
+int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream);
+
 }  // namespace fd
