@@ -36,10 +36,11 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& p, int tile, int r
     int before = 0;
     LoraTile f{-2, 0, 0};
     for (int base = 0; base < p.n_seg; base += 32) {
-        int lo = 0, n = 0;
+        int lo = 0, n = 0, id = -1;
         if (base + lane < p.n_seg) {
             lo = p.start[base + lane];
             const int hi = p.start[base + lane + 1];
+            id = p.ids[base + lane];
             n = hi - lo;
             if (lo < 0 || n < 0 || hi > p.T) { set_status(p.status, STATUS_BAD_INDEX); n = 0; }
         }
@@ -56,7 +57,7 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& p, int tile, int r
             const int skipped = tile - before - __shfl_sync(0xffffffffu, sum - tiles, src);
             f.begin = __shfl_sync(0xffffffffu, lo, src) + skipped * rows;
             f.count = min(rows, __shfl_sync(0xffffffffu, n, src) - skipped * rows);
-            f.adapter = p.ids[base + src];
+            f.adapter = __shfl_sync(0xffffffffu, id, src);
             if (f.adapter < -1 || f.adapter >= p.E) {
                 set_status(p.status, STATUS_BAD_INDEX);
                 f.adapter = -2;
