@@ -3,30 +3,44 @@
 //     c(b, v) = s_b + x(b, v) - lse_b,      lse_b = log sum_v exp x(b, v),
 // and the k best of a request by (c descending, (b - first) V + v ascending) are wanted.
 //
-// Two kernels.  The first streams the logits once: per row the pieces of the normaliser, and per group of 128 neighbouring
-// entries their largest value.  Nothing else of the row has to be looked at again: if T is a number that at least k groups'
-// maxima reach, every one of the k best reaches T and lies in a group whose maximum does, and those groups are k or a few more of the
-// thousands.  The second kernel, one CTA per request, finds such a T, reads those groups again and ranks what reaches T.
+// The logits are read once: per row the pieces of the normaliser, and per group of 128 neighbouring entries their largest
+// value.  Nothing else of the row has to be looked at again: if T is a number that at least k groups' maxima reach, every one
+// of the k best reaches T and lies in a group whose maximum does, and those groups are k or a few more of the thousands.  One CTA per
+// request finds such a T, reads those groups again and ranks what reaches T.
+//
+// Two forms.  Few bytes per request: a thread-block cluster per request reads them, leaves the maxima in its shared memory, and its first
+// CTA picks from there - one launch, no memory in between.  More: one kernel streams all rows with the whole GPU, a second one picks
+// (the clusters' other CTAs would hold their SMs while the first ones pick).
 //
 // Why the sums are in 64 bits: which of two candidates of different beams comes first hangs on the difference of two
 // normalisers.  In 32 bits they are off by some 1e-6, and among the candidates of a large batch two that are nearer than
 // that are common (gaps of 1e-2 between neighbours: one pair in ten thousand, and a step of 64 requests has a thousand pairs).  The
-// exponentials themselves are taken in 32 bits of differences that are exact or off by half a step; their errors of 1e-7 have no
-// common sign and average out over the row.  Groups of 16 are added in 32 bits, then in 64.
+// exponentials themselves are taken in 32 bits, 2^(d log2 e) of differences d = x - max that are exact or off by half a step, with log2 e as
+// the sum of two numbers (one alone is off by 2^-26 of itself, the same way for every entry); what errors of 1e-7 are left have
+// no common sign and average out over the row.  Groups of 16 are added in 32 bits, then in 64.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include "common.cuh"
 
 namespace fd {
 
-constexpr int BM_GROUP = 128;            // entries per group: four coalesced loads of a warp
-constexpr int BM_BATCH = 4;              // groups that a warp has in flight at once
+namespace cg = cooperative_groups;
+
+// Entries per group: 128, four coalesced loads of a warp, or 32, one, for small vocabularies: what reaches T comes from few rows
+// where the beams' scores are far apart, and T is only as near the k-th best as those rows' groups are many.
+constexpr int BM_GROUP = 128, BM_SMALL_GROUP = 32;
+constexpr int BM_SMALL_VOCAB = 16384;
+constexpr int BM_UNIT = 128;             // entries that a warp takes at a time
+constexpr int BM_BATCH = 4;              // such units that a warp has in flight at once
 constexpr int BM_SCAN_THREADS = 256, BM_SCAN_WARPS = BM_SCAN_THREADS / 32;
-constexpr int BM_PICK_THREADS = 1024, BM_PICK_WARPS = BM_PICK_THREADS / 32;
+constexpr int BM_PICK_THREADS = 1024;
+constexpr int BM_CLUSTER_THREADS = 512;
 constexpr int BM_MAX_ROWS = 64;          // beams of one request
 constexpr int BM_MAX_K = 128;            // candidates of one request
 constexpr int BM_LIST = 512;             // groups that may reach T before the exact cut is taken
 constexpr int BM_FOUND = 2048;           // entries that may
+constexpr int BM_KEPT = 256;             // entries that are ranked (more than that many get a nearer threshold first)
 
 __device__ __forceinline__ float warp_max_redux(float v) {
     float r;
@@ -34,83 +48,136 @@ __device__ __forceinline__ float warp_max_redux(float v) {
     return r;
 }
 
-// How a row's groups are dealt to CTAs: `per` groups (a multiple of what the CTA's warps have in flight) for each of `splits`.
+// How a row's units are dealt to CTAs: `per` units (a multiple of what the CTA's warps have in flight) for each of `splits`.
 struct BeamPlan {
-    int groups, per, splits;
+    int units, per, splits;
 };
 static BeamPlan beam_plan(int n, int V) {
     BeamPlan p;
     constexpr int unit = BM_SCAN_WARPS * BM_BATCH;
-    p.groups = (V + BM_GROUP - 1) / BM_GROUP;
-    const long long total = (long long)n * p.groups;
+    p.units = (V + BM_UNIT - 1) / BM_UNIT;
+    const long long total = (long long)n * p.units;
     const long long want = (total + 148 * 16 - 1) / (148 * 16);          // two waves of eight CTAs per SM
     const long long per = ((want + unit - 1) / unit) * unit;
     p.per = (int)(per < unit ? unit : per);
-    if (p.per > p.groups) p.per = ((p.groups + unit - 1) / unit) * unit;
-    p.splits = (p.groups + p.per - 1) / p.per;
+    if (p.per > p.units) p.per = ((p.units + unit - 1) / unit) * unit;
+    p.splits = (p.units + p.per - 1) / p.per;
     return p;
 }
 
-__global__ void __launch_bounds__(BM_SCAN_THREADS)
-beam_scan_kernel(const float* __restrict__ logits, int V, int groups, int per, float* __restrict__ gmax, float* __restrict__ part_m,
-                 double* __restrict__ part_s) {
-    const int row = blockIdx.y, split = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float* x = logits + (size_t)row * V;
-    float* gm = gmax + (size_t)row * groups;
-    const int end = min(groups, (split + 1) * per);
-    float m = -INFINITY;                 // the warp's running maximum, the same in all lanes
-    double s = 0.0;                      // this lane's sum of exp(x - m)
+// exp(d) for d <= 0, off by about 2^-22 of itself at most; 0 for -inf.
+__device__ __forceinline__ float beam_exp(float d) {
+    constexpr float LOG2E_HI = 1.44269502162933349609375f;       // log2 e rounded down, and what is left of it
+    constexpr float LOG2E_LO = 1.92596299112661746887e-8f;
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(d, LOG2E_LO, d * LOG2E_HI)));
+    return r;
+}
+
+// A warp's share of one row: units g, g + stride, ... of those before `end`, BM_BATCH neighbours at a time.  The maxima of their groups
+// go to gm[group]; (m, s): the largest value (the same in all lanes) and this lane's sum of exp(x - m).
+// VEC: a lane has four neighbours (rows that are a multiple of four, 16-byte aligned), else every 32nd.  SMALL: groups of 32.
+template <bool VEC, bool SMALL>
+__device__ __forceinline__ void beam_scan_row(const float* __restrict__ x, int V, int g, int end, int stride, float* gm, float& m, double& s) {
+    const int lane = threadIdx.x & 31;
     float v[BM_BATCH][4], nxt[BM_BATCH][4];
     auto fetch = [&](int g0, float (&d)[BM_BATCH][4]) {
+        if (g0 + BM_BATCH <= end && (g0 + BM_BATCH) * BM_UNIT <= V) {           // whole groups: no check per entry
+            const float* p = x + (size_t)g0 * BM_UNIT;
 #pragma unroll
-        for (int j = 0; j < BM_BATCH; ++j)
+            for (int j = 0; j < BM_BATCH; ++j) {
+                if (VEC) {
+                    const float4 q = __ldcs(reinterpret_cast<const float4*>(p + j * BM_UNIT) + lane);
+                    d[j][0] = q.x; d[j][1] = q.y; d[j][2] = q.z; d[j][3] = q.w;
+                } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = (g0 + j) * BM_GROUP + e * 32 + lane;
-                d[j][e] = (g0 + j < end && i < V) ? __ldg(x + i) : -INFINITY;
+                    for (int e = 0; e < 4; ++e) d[j][e] = __ldcs(p + j * BM_UNIT + e * 32 + lane);
+                }
             }
-    };
-    int g0 = split * per + warp * BM_BATCH;
-    fetch(g0, v);
-    for (; g0 < end; g0 += BM_SCAN_WARPS * BM_BATCH) {
-        fetch(g0 + BM_SCAN_WARPS * BM_BATCH, nxt);
-        float best[BM_BATCH], top = -INFINITY;
+        } else {
 #pragma unroll
-        for (int j = 0; j < BM_BATCH; ++j) {
-            best[j] = warp_max_redux(fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
-            if (lane == j && g0 + j < end) gm[g0 + j] = best[j];
-            top = fmaxf(top, best[j]);
+            for (int j = 0; j < BM_BATCH; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = (g0 + j) * BM_UNIT + (VEC ? lane * 4 + e : e * 32 + lane);
+                    d[j][e] = g0 + j < end && i < V ? __ldcs(x + i) : -INFINITY;
+                }
+        }
+    };
+    if (g < end) fetch(g, v);
+    for (; g < end; g += stride) {
+        if (g + stride < end) fetch(g + stride, nxt);
+        float top = -INFINITY, kept = -INFINITY;                 // lane i keeps the i-th maximum
+        if (SMALL) {
+#pragma unroll
+            for (int j = 0; j < BM_BATCH; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float best = warp_max_redux(v[j][e]);
+                    top = fmaxf(top, best);
+                    if (lane == j * 4 + e) kept = best;
+                }
+            if (lane < BM_BATCH * 4 && g + lane / 4 < end && (g * 4 + lane) * BM_SMALL_GROUP < V) gm[g * 4 + lane] = kept;
+        } else {
+#pragma unroll
+            for (int j = 0; j < BM_BATCH; ++j) {
+                const float best = warp_max_redux(fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+                top = fmaxf(top, best);
+                if (lane == j) kept = best;
+            }
+            if (lane < BM_BATCH && g + lane < end) gm[g + lane] = kept;
         }
         if (top > m) {                   // warp-uniform, and rare after the first few batches
-            s *= (double)expf(m - top);  // m = -inf: times 0
+            s *= (double)beam_exp(m - top);                      // m = -inf: times 0
             m = top;
         }
-        const float mm = m == -INFINITY ? 0.f : m;          // nothing but -inf so far: every exp below is 0, not NaN
+        const float mm = m == -INFINITY ? 0.f : m;               // nothing but -inf so far: every exp below is 0, not NaN
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < BM_BATCH; ++j)
-            sum += (expf(v[j][0] - mm) + expf(v[j][1] - mm)) + (expf(v[j][2] - mm) + expf(v[j][3] - mm));
+            sum += (beam_exp(v[j][0] - mm) + beam_exp(v[j][1] - mm)) + (beam_exp(v[j][2] - mm) + beam_exp(v[j][3] - mm));
         s += (double)sum;
 #pragma unroll
         for (int j = 0; j < BM_BATCH; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[j][e] = nxt[j][e];
     }
+}
+
+// (m, s) of the CTA's warps as one, in thread 0.
+template <int WARPS>
+__device__ __forceinline__ void beam_join(float& m, double& s, float* sm, double* ss) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    __shared__ float sm[BM_SCAN_WARPS];
-    __shared__ double ss[BM_SCAN_WARPS];
     if (lane == 0) { sm[warp] = m; ss[warp] = s; }
     __syncthreads();
+    if (warp == 0) {
+        m = lane < WARPS ? sm[lane] : -INFINITY;
+        s = lane < WARPS ? ss[lane] : 0.0;
+        const float M = warp_max(m);
+        if (m != -INFINITY) s *= exp((double)m - (double)M);     // else 0, or NaN
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        m = M;
+    }
+}
+
+template <bool VEC, bool SMALL>
+__global__ void __launch_bounds__(BM_SCAN_THREADS)
+beam_scan_kernel(const float* __restrict__ logits, int V, int units, int groups, int per, float* __restrict__ gmax, float* __restrict__ part_m,
+                 double* __restrict__ part_s) {
+    const int row = blockIdx.y, split = blockIdx.x, warp = threadIdx.x >> 5;
+    float m = -INFINITY;
+    double s = 0.0;
+    beam_scan_row<VEC, SMALL>(logits + (size_t)row * V, V, split * per + warp * BM_BATCH, min(units, (split + 1) * per), BM_SCAN_WARPS * BM_BATCH,
+                       gmax + (size_t)row * groups, m, s);
+    __shared__ float sm[BM_SCAN_WARPS];
+    __shared__ double ss[BM_SCAN_WARPS];
+    beam_join<BM_SCAN_WARPS>(m, s, sm, ss);
     if (threadIdx.x == 0) {
-        float M = -INFINITY;
-        for (int w = 0; w < BM_SCAN_WARPS; ++w) M = fmaxf(M, sm[w]);
-        double S = 0.0;
-        for (int w = 0; w < BM_SCAN_WARPS; ++w)
-            if (sm[w] != -INFINITY) S += ss[w] * exp((double)sm[w] - (double)M);
-            else S += ss[w];             // 0, or NaN
-        part_m[(size_t)row * gridDim.x + split] = M;
-        part_s[(size_t)row * gridDim.x + split] = S;
+        part_m[(size_t)row * gridDim.x + split] = m;
+        part_s[(size_t)row * gridDim.x + split] = s;
     }
 }
 
@@ -126,205 +193,367 @@ __device__ __forceinline__ double beam_value(unsigned long long key) {
     return __longlong_as_double((long long)((key >> 63) ? (key & 0x7fffffffffffffffull) : ~key));
 }
 
+template <int THREADS>
 __device__ __forceinline__ int block_total(int v, int* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     v = __reduce_add_sync(0xffffffffu, v);
     if (lane == 0) scratch[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        const int t = __reduce_add_sync(0xffffffffu, scratch[lane]);
-        if (lane == 0) scratch[BM_PICK_WARPS] = t;
+        const int t = __reduce_add_sync(0xffffffffu, lane < THREADS / 32 ? scratch[lane] : 0);
+        if (lane == 0) scratch[32] = t;
     }
     __syncthreads();
-    const int t = scratch[BM_PICK_WARPS];
+    const int t = scratch[32];
     __syncthreads();
     return t;
 }
 
 // The exact cut: of the items 0 .. n - 1 with keys key(i) (0: none) those that are among the k first by (key descending, i
 // ascending) are the ones with key > T, or key == T and i <= I.  Found bit by bit, each bit a count over all items.
-template <typename Key>
+template <int THREADS, typename Key>
 __device__ void exact_cut(int n, int k, Key key, unsigned long long& T, int& I, int* scratch) {
     T = 0ull;
     for (int bit = 63; bit >= 0; --bit) {
         const unsigned long long t = T | (1ull << bit);
         int c = 0;
-        for (int i = threadIdx.x; i < n; i += BM_PICK_THREADS) c += key(i) >= t;
-        if (block_total(c, scratch) >= k) T = t;
+        for (int i = threadIdx.x; i < n; i += THREADS) c += key(i) >= t;
+        if (block_total<THREADS>(c, scratch) >= k) T = t;
     }
     I = 0x7fffffff;
     if (T == 0ull) { T = 1ull; return; }                       // fewer than k candidates: all of them
     int c = 0;
-    for (int i = threadIdx.x; i < n; i += BM_PICK_THREADS) c += key(i) > T;
-    const int need = k - block_total(c, scratch);              // of those equal to T, the first so many
+    for (int i = threadIdx.x; i < n; i += THREADS) c += key(i) > T;
+    const int need = k - block_total<THREADS>(c, scratch);              // of those equal to T, the first so many
     int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = lo + (hi - lo) / 2;
         c = 0;
-        for (int i = threadIdx.x; i <= mid; i += BM_PICK_THREADS) c += key(i) == T;
-        if (block_total(c, scratch) >= need) hi = mid; else lo = mid + 1;
+        for (int i = threadIdx.x; i <= mid; i += THREADS) c += key(i) == T;
+        if (block_total<THREADS>(c, scratch) >= need) hi = mid; else lo = mid + 1;
     }
     I = lo;
 }
 
-// One CTA per request.
-__global__ void __launch_bounds__(BM_PICK_THREADS)
-beam_pick_kernel(const float* __restrict__ logits, int V, int n, const float* __restrict__ scores, const int* __restrict__ start,
-                 int groups, int splits, const float* __restrict__ gmax, const float* __restrict__ part_m,
-                 const double* __restrict__ part_s, int k, float* __restrict__ out_s, int* __restrict__ out_row,
-                 int* __restrict__ out_tok, int* status) {
-    __shared__ double2 off[BM_MAX_ROWS];
-    __shared__ int list[BM_LIST];
-    __shared__ unsigned long long fkey[BM_FOUND];
-    __shared__ int fidx[BM_FOUND];
-    __shared__ int scratch[BM_PICK_WARPS + 1];
-    __shared__ int n_list, n_found;
-    const int r = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int first = start[r], last = start[r + 1];
-    const bool good = first >= 0 && last >= first && last <= n && last - first <= BM_MAX_ROWS;
-    const int nb = good ? last - first : 0;
-    if (!good && t == 0) set_status(status, STATUS_BAD_INDEX);
-    for (int j = t; j < k; j += BM_PICK_THREADS) {             // what is not found stays so
-        out_s[(size_t)r * k + j] = -INFINITY;
-        out_row[(size_t)r * k + j] = -1;
-        out_tok[(size_t)r * k + j] = -1;
-    }
-    if (t == 0) { n_list = 0; n_found = 0; }
-    // a row whose score or normaliser is no finite number has no candidates
-    for (int b = warp; b < nb; b += BM_PICK_WARPS) {
-        const size_t p = (size_t)(first + b) * splits;
-        float M = -INFINITY;
-        for (int i = lane; i < splits; i += 32) M = fmaxf(M, part_m[p + i]);
-        M = warp_max(M);
-        double S = 0.0;
-        for (int i = lane; i < splits; i += 32) {
-            const float mi = part_m[p + i];
-            S += mi == -INFINITY ? part_s[p + i] : part_s[p + i] * exp((double)mi - (double)M);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
-        if (lane == 0) {
-            const double o = (double)scores[first + b] - log(S);
-            const bool fine = isfinite(o) && isfinite(M);
-            off[b] = make_double2(fine ? (double)M : 0.0, fine ? o : -(double)INFINITY);       // or every key of the row is 0
-        }
-    }
-    __syncthreads();
-    if (nb == 0) return;
+// What one CTA does for a request once the logits have been read.  off[b]: (max, s_b - log sum exp(x - max)) of its rows; the maxima of
+// its groups lie in pieces: piece c, at at(c), has groups c * seg .. of every row, [rows][seg].
+struct BeamShared {
+    double2 off[BM_MAX_ROWS];
+    unsigned long long fkey[BM_FOUND], key[BM_KEPT];
+    int fidx[BM_FOUND], idx[BM_KEPT];
+    int list[BM_LIST];
+    int scratch[33];
+    int n_list, n_found, n_kept;
+};
+struct BeamOut {
+    float* score;
+    int* row;
+    int* tok;
+};
 
-    const float* gm = gmax + (size_t)first * groups;           // the request's groups, one after another
-    const float* x = logits + (size_t)first * V;
-    const int N = nb * groups;
-    auto group_key = [&](int i) { return beam_key(off[i / groups], gm[i]); };
-    unsigned long long mine = 0ull;
-    for (int i = t; i < N; i += BM_PICK_THREADS) {
-        const unsigned long long q = group_key(i);
-        mine = q > mine ? q : mine;
+// Division of small numbers (quotient and divisor below 2^16) by a number that is not known to the compiler: exact, since the quotient's
+// error in 32 bits is far below the distance of (i + 1/2) / d from a whole number.
+struct BeamDiv {
+    float inv;
+    int d;
+    __device__ __forceinline__ explicit BeamDiv(int v) : inv(1.f / (float)v), d(v) {}
+    __device__ __forceinline__ int operator()(int i) const { return (int)(((float)i + 0.5f) * inv); }
+};
+template <typename At>
+struct BeamMaxima {
+    BeamDiv row, piece;
+    At at;
+    __device__ __forceinline__ float operator()(int i, int& b) const {
+        b = row(i);
+        const int g = i - b * row.d, c = piece(g);
+        return at(c)[b * piece.d + g - c * piece.d];
     }
-    // T: at least k of the threads' maxima reach it (or all candidates do); a few more than k will do
-    unsigned long long T = 0ull;
-    if (__syncthreads_count(mine != 0ull) >= k) {
-        for (int bit = 63; bit >= 0; --bit) {
-            const unsigned long long q = T | (1ull << bit);
-            const int c = __syncthreads_count(mine >= q);
-            if (c >= k) {
-                T = q;
-                if (c <= k + k / 4 + 2) break;
-            }
-        }
+};
+
+__device__ __forceinline__ void beam_none(const BeamOut& out, int r, int k) {     // what is not found stays so
+    for (int j = threadIdx.x; j < k; j += blockDim.x) {
+        out.score[(size_t)r * k + j] = -INFINITY;
+        out.row[(size_t)r * k + j] = -1;
+        out.tok[(size_t)r * k + j] = -1;
     }
-    if (T == 0ull) T = 1ull;
-    for (int i = t; i < N; i += BM_PICK_THREADS)
-        if (group_key(i) >= T) {
-            const int at = atomicAdd(&n_list, 1);
-            if (at < BM_LIST) list[at] = i;
-        }
-    __syncthreads();
-    int ng = n_list;
-    unsigned long long cut = T;
-    bool listed = ng <= BM_LIST;
-    if (listed) {
-        for (int j = warp; j < ng; j += BM_PICK_WARPS) {
-            const int i = list[j], b = i / groups, v0 = (i - b * groups) * BM_GROUP;
+}
+
+// A row's pieces (m, s) are added up; a row whose score or normaliser is no finite number has no candidates.  Called by a warp.
+template <typename Piece>
+__device__ __forceinline__ double2 beam_offset(float score, int pieces, Piece piece) {
+    const int lane = threadIdx.x & 31;
+    float M = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) M = fmaxf(M, piece(i).x);
+    M = warp_max(M);
+    double S = 0.0;
+    for (int i = lane; i < pieces; i += 32) {
+        const double2 p = piece(i);
+        S += p.x == -INFINITY ? p.y : p.y * exp(p.x - (double)M);
+    }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = v0 + e * 32 + lane;
-                const unsigned long long q = v < V ? beam_key(off[b], x[(size_t)b * V + v]) : 0ull;
+    for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
+    const double o = (double)score - log(S);
+    const bool fine = isfinite(o) && isfinite(M);
+    return make_double2(fine ? (double)M : 0.0, fine ? o : -(double)INFINITY);               // -inf: every key of the row is 0
+}
+
+// A number that at least k of the threads' `keys` (N of them each, 0: none) reach, and hardly more; 1 where there are fewer than k.
+template <int N>
+__device__ __forceinline__ unsigned long long beam_threshold(const unsigned long long (&keys)[N], int k) {
+    auto reach = [&](unsigned long long q) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __syncthreads_count(keys[i] >= q);
+        return c;
+    };
+    if (reach(1ull) < k) return 1ull;
+    unsigned long long T = 0ull;
+    for (int bit = 63; bit >= 0; --bit) {
+        const unsigned long long q = T | (1ull << bit);
+        const int c = reach(q);
+        if (c >= k) {
+            T = q;
+            if (c <= k + k / 4 + 2) break;
+        }
+    }
+    return T;
+}
+
+template <int THREADS, int GROUP, typename At>
+__device__ void beam_pick(BeamShared& sh, const float* __restrict__ x, int V, int groups, int nb, int first, int seg, At at, int k, int r,
+                          const BeamOut& out) {
+    constexpr int WARPS = THREADS / 32;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int N = nb * groups;
+    const BeamMaxima<At> maxima{BeamDiv(groups), BeamDiv(seg), at};
+    auto group_key = [&](int i) {
+        int b;
+        const float v = maxima(i, b);
+        return beam_key(sh.off[b], v);
+    };
+    if (t == 0) sh.n_list = sh.n_found = sh.n_kept = 0;
+    unsigned long long mine[1] = {0ull};
+#pragma unroll 4
+    for (int i = t; i < N; i += THREADS) {
+        const unsigned long long q = group_key(i);
+        mine[0] = q > mine[0] ? q : mine[0];
+    }
+    unsigned long long T = beam_threshold(mine, k);
+    if (mine[0] >= T)
+        for (int i = t; i < N; i += THREADS)
+            if (group_key(i) >= T) {
+                const int p = atomicAdd(&sh.n_list, 1);
+                if (p < BM_LIST) sh.list[p] = i;
+            }
+    __syncthreads();
+    int ng = sh.n_list;
+    const bool listed = ng <= BM_LIST;
+    constexpr int EACH = GROUP / 32;                             // entries of a group per lane
+    if (listed) {
+        for (int j = warp; j < ng; j += WARPS) {
+            const int i = sh.list[j], b = maxima.row(i), v0 = (i - b * groups) * GROUP;
+            float e[EACH];
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) e[u] = v0 + u * 32 + lane < V ? __ldg(x + (size_t)b * V + v0 + u * 32 + lane) : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) {
+                const unsigned long long q = beam_key(sh.off[b], e[u]);
                 if (q >= T) {
-                    const int at = atomicAdd(&n_found, 1);
-                    if (at < BM_FOUND) { fkey[at] = q; fidx[at] = b * V + v; }
+                    const int p = atomicAdd(&sh.n_found, 1);
+                    if (p < BM_FOUND) { sh.fkey[p] = q; sh.fidx[p] = b * V + v0 + u * 32 + lane; }
                 }
             }
         }
     }
     __syncthreads();
-    if (!listed || n_found > BM_FOUND) {
+    const unsigned long long* key = sh.fkey;
+    const int* idx = sh.fidx;
+    int nf = sh.n_found;
+    bool exact = !listed || nf > BM_FOUND;
+    if (!exact && nf > BM_KEPT) {
+        // a nearer threshold, from the entries themselves
+        unsigned long long own[BM_FOUND / THREADS];
+#pragma unroll
+        for (int u = 0; u < BM_FOUND / THREADS; ++u) own[u] = t + u * THREADS < nf ? sh.fkey[t + u * THREADS] : 0ull;
+        const unsigned long long T2 = beam_threshold(own, k);
+#pragma unroll
+        for (int u = 0; u < BM_FOUND / THREADS; ++u)
+            if (own[u] >= T2 && own[u] != 0ull) {
+                const int p = atomicAdd(&sh.n_kept, 1);
+                if (p < BM_KEPT) { sh.key[p] = own[u]; sh.idx[p] = sh.fidx[t + u * THREADS]; }
+            }
+        __syncthreads();
+        key = sh.key;
+        idx = sh.idx;
+        nf = sh.n_kept;
+        exact = nf > BM_KEPT;
+    }
+    if (exact) {
         // Too many entries reach T: rows that are constant, or nearly.  The k best lie in the k best groups (by maximum, then by
         // place: each of k better groups holds an entry that is better than any of a group behind them), and there are at most
         // k x 128 entries in those; both cuts are exact.
         int I;
-        exact_cut(N, k, group_key, T, I, scratch);
-        if (t == 0) { n_list = 0; n_found = 0; }
+        exact_cut<THREADS>(N, k, group_key, T, I, sh.scratch);
+        if (t == 0) sh.n_list = sh.n_kept = 0;
         __syncthreads();
-        for (int i = t; i < N; i += BM_PICK_THREADS) {
+        for (int i = t; i < N; i += THREADS) {
             const unsigned long long q = group_key(i);
-            if (q > T || (q == T && i <= I)) list[atomicAdd(&n_list, 1)] = i;          // k at most
+            if (q > T || (q == T && i <= I)) sh.list[atomicAdd(&sh.n_list, 1)] = i;          // k at most
         }
         __syncthreads();
-        ng = n_list;
+        ng = sh.n_list;
         // in the order of their places, so that an entry's number among them orders like its own place
-        int at = 0, own = 0;
+        int place = 0, own = 0;
         if (t < ng) {
-            own = list[t];
-            for (int j = 0; j < ng; ++j) at += list[j] < own;
+            own = sh.list[t];
+            for (int j = 0; j < ng; ++j) place += sh.list[j] < own;
         }
         __syncthreads();
-        if (t < ng) list[at] = own;
+        if (t < ng) sh.list[place] = own;
         __syncthreads();
-        auto entry_key = [&](int i) {
-            const int g = list[i / BM_GROUP], b = g / groups, v = (g - b * groups) * BM_GROUP + i % BM_GROUP;
-            return v < V ? beam_key(off[b], x[(size_t)b * V + v]) : 0ull;
+        auto entry = [&](int i, int& b) {
+            const int g = sh.list[i / GROUP];
+            b = maxima.row(g);
+            return (g - b * groups) * GROUP + i % GROUP;
         };
-        exact_cut(ng * BM_GROUP, k, entry_key, cut, I, scratch);
-        for (int i = t; i < ng * BM_GROUP; i += BM_PICK_THREADS) {
+        auto entry_key = [&](int i) {
+            int b;
+            const int v = entry(i, b);
+            return v < V ? beam_key(sh.off[b], x[(size_t)b * V + v]) : 0ull;
+        };
+        unsigned long long cut;
+        exact_cut<THREADS>(ng * GROUP, k, entry_key, cut, I, sh.scratch);
+        for (int i = t; i < ng * GROUP; i += THREADS) {
             const unsigned long long q = entry_key(i);
             if (q > cut || (q == cut && i <= I)) {
-                const int g = list[i / BM_GROUP], b = g / groups;
-                const int p = atomicAdd(&n_found, 1);                                  // k at most
-                fkey[p] = q;
-                fidx[p] = b * V + (g - b * groups) * BM_GROUP + i % BM_GROUP;
+                int b;
+                const int v = entry(i, b), p = atomicAdd(&sh.n_kept, 1);                     // k at most
+                sh.key[p] = q;
+                sh.idx[p] = b * V + v;
             }
         }
         __syncthreads();
+        key = sh.key;
+        idx = sh.idx;
+        nf = sh.n_kept;
     }
     // an entry's place is the number of entries before it
-    const int nf = n_found;
-    for (int j = t; j < nf; j += BM_PICK_THREADS) {
-        const unsigned long long q = fkey[j];
-        const int id = fidx[j];
+    for (int j = t; j < nf; j += THREADS) {
+        const unsigned long long q = key[j];
+        const int id = idx[j];
         int rank = 0;
         for (int i = 0; i < nf; ++i) {
-            const unsigned long long o = fkey[i];
-            rank += o > q || (o == q && fidx[i] < id);
+            const unsigned long long o = key[i];
+            rank += o > q || (o == q && idx[i] < id);
         }
         if (rank < k) {
             const size_t p = (size_t)r * k + rank;
-            out_s[p] = (float)beam_value(q);
-            out_row[p] = first + id / V;
-            out_tok[p] = id % V;
+            out.score[p] = (float)beam_value(q);
+            out.row[p] = first + id / V;
+            out.tok[p] = id % V;
         }
     }
+}
+
+// The rows of request r; none (and a report) where the range is no range.
+__device__ __forceinline__ int beam_rows(const int* start, int r, int n, int& first, int* status) {
+    first = start[r];
+    const int last = start[r + 1];
+    if (first >= 0 && last >= first && last <= n && last - first <= BM_MAX_ROWS) return last - first;
+    if (threadIdx.x == 0) set_status(status, STATUS_BAD_INDEX);
+    return 0;
+}
+
+// One CTA per request, behind the scan.
+template <int GROUP>
+__global__ void __launch_bounds__(BM_PICK_THREADS)
+beam_pick_kernel(const float* __restrict__ logits, int V, int n, const float* __restrict__ scores, const int* __restrict__ start,
+                 int groups, int splits, const float* __restrict__ gmax, const float* __restrict__ part_m,
+                 const double* __restrict__ part_s, int k, const BeamOut out, int* status) {
+    __shared__ BeamShared sh;
+    const int r = blockIdx.x;
+    int first;
+    const int nb = beam_rows(start, r, n, first, status);
+    beam_none(out, r, k);
+    for (int b = threadIdx.x >> 5; b < nb; b += BM_PICK_THREADS / 32) {
+        const size_t p = (size_t)(first + b) * splits;
+        const double2 o = beam_offset(scores[first + b], splits, [&](int i) { return make_double2(part_m[p + i], part_s[p + i]); });
+        if ((threadIdx.x & 31) == 0) sh.off[b] = o;
+    }
+    __syncthreads();
+    if (nb == 0) return;
+    const float* gm = gmax + (size_t)first * groups;           // the request's groups, one after another
+    beam_pick<BM_PICK_THREADS, GROUP>(sh, logits + (size_t)first * V, V, groups, nb, first, groups, [&](int) { return gm; }, k, r, out);
+}
+
+// One cluster per request: each CTA has the same part of every row, each warp the same part of that (so that equal rows have equal
+// normalisers, to the bit); the first CTA picks.
+template <bool VEC, bool SMALL>
+__global__ void __launch_bounds__(BM_CLUSTER_THREADS)
+beam_cluster_kernel(const float* __restrict__ logits, int V, int n, const float* __restrict__ scores, const int* __restrict__ start,
+                    int units, int groups, int k, const BeamOut out, int* status) {
+    constexpr int WARPS = BM_CLUSTER_THREADS / 32;
+    extern __shared__ float gm[];                              // [rows][seg]: the maxima of this CTA's groups
+    __shared__ BeamShared sh;
+    __shared__ double2 parts[BM_MAX_ROWS * WARPS];             // (m, s) of each warp's part of each row
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = cluster.num_blocks(), rank = cluster.block_rank(), r = blockIdx.x / C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    int first;
+    const int nb = beam_rows(start, r, n, first, status);
+    if (rank == 0) beam_none(out, r, k);
+    if (nb == 0) return;                                       // the same for the whole cluster
+    const int per = (units + C - 1) / C, u0 = rank * per, u1 = min(units, u0 + per);
+    constexpr int GROUP = SMALL ? BM_SMALL_GROUP : BM_GROUP;
+    const int seg = per * (BM_UNIT / GROUP);                   // groups of a part
+    int per_row = 1;                                           // warps that share a row: no more than have work, all rows at once
+    while (2 * per_row * nb <= WARPS && per_row * BM_BATCH < per) per_row *= 2;
+    for (int b = warp / per_row; b < nb; b += WARPS / per_row) {
+        float m = -INFINITY;
+        double s = 0.0;
+        beam_scan_row<VEC, SMALL>(logits + (size_t)(first + b) * V, V, u0 + (warp % per_row) * BM_BATCH, u1, per_row * BM_BATCH, gm + b * seg - rank * seg, m, s);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) parts[b * per_row + warp % per_row] = make_double2(m, s);
+    }
+    cluster.sync();
+    if (rank == 0) {
+        for (int b = warp; b < nb; b += WARPS) {
+            const double2 o = beam_offset(scores[first + b], C * per_row,
+                                          [&](int i) { return *cluster.map_shared_rank(parts + b * per_row + i % per_row, i / per_row); });
+            if (lane == 0) sh.off[b] = o;
+        }
+        __syncthreads();
+        beam_pick<BM_CLUSTER_THREADS, GROUP>(sh, logits + (size_t)first * V, V, groups, nb, first, seg,
+                                      [&](int c) { return (const float*)cluster.map_shared_rank(gm, c); }, k, r, out);
+    }
+    cluster.sync();                                            // the maxima have been read
 }
 
 }  // namespace fd
 
 using namespace fd;
 
+// Bytes of logits per CTA up to which the one launch is taken.  Measured, clusters / two kernels, us on the device and the host's time of a
+// call (11 / 15 us, the more of the two when calls follow each other): 4 rows of 151,936 (152 KB per CTA) 13.7 / 11.1; 36 ragged
+// rows of 50,257 for 7 requests (65 KB) 13.6 / 12.2; 106 rows of 2,410 for 53 8.7 / 9.5; but 3 requests of up to 28 rows of 82,102
+// (270 KB) 33 / 21, 512 rows of 152,064 for 64 95 / 65.
+constexpr long long BM_CLUSTER_BYTES = 160 * 1024;
+
 // Bytes of scratch that fd_beam_select needs for n rows of V logits (8-byte aligned).
 extern "C" long long fd_beam_select_scratch_bytes(int n, int V) {
     if (n <= 0 || V <= 0) return 0;
     const BeamPlan p = beam_plan(n, V);
-    return (long long)n * p.splits * 12 + (long long)n * p.groups * 4;
+    return (long long)n * p.splits * 12 + (long long)n * p.units * (V <= BM_SMALL_VOCAB ? 16 : 4);
+}
+
+extern "C" int fd_sm_count();
+
+static int g_beam_form = 0;
+// Which form fd_beam_select takes from now on: 1 = a cluster per request (where its memory suffices), 2 = two kernels, 0 = by the sizes.
+// For tests and measurements.
+extern "C" int fd_beam_select_set_form(int form) {
+    g_beam_form = form;
+    return 0;
 }
 
 // logits [n, V], scores [n] float; start [R + 1] int: request r has the rows start[r] .. start[r + 1] - 1, at most 64.  Out [R, k].
@@ -335,14 +564,42 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     FD_REQUIRE(n <= 65535, -2, "beam_select: %d rows in one call", n);
     FD_REQUIRE(k >= 1 && k <= BM_MAX_K, -2, "beam_select: %d candidates per request; 1 to %d are taken", k, BM_MAX_K);
     FD_REQUIRE((long long)V * BM_MAX_ROWS < (1ll << 31), -2, "beam_select: a vocabulary of %d", V);
+    const BeamOut out{out_s, out_row, out_tok};
+    const bool small = V <= BM_SMALL_VOCAB;
+    const bool vec = !small && V % 4 == 0 && (reinterpret_cast<unsigned long long>(logits) & 15) == 0;
+    const int sms = fd_sm_count(), units = (V + BM_UNIT - 1) / BM_UNIT, size = small ? BM_SMALL_GROUP : BM_GROUP, groups = (V + size - 1) / size;
+    int C = 16;
+    while (C > 1 && (R * C > 2 * sms || units < C)) C /= 2;
+    // (a request may have all the rows, up to 64)
+    const long long smem = 4ll * (n < BM_MAX_ROWS ? n : BM_MAX_ROWS) * ((units + C - 1) / C) * (BM_UNIT / size);
+    const bool fits = smem <= 96 * 1024 && R <= 2 * sms;
+    if (fits && g_beam_form != 2 && (g_beam_form == 1 || 4ll * n * V <= BM_CLUSTER_BYTES * R * C)) {
+        const int which = small ? 2 : (vec ? 1 : 0);
+        void (*const kernels[3])(const float*, int, int, const float*, const int*, int, int, int, const BeamOut, int*) = {
+            beam_cluster_kernel<false, false>, beam_cluster_kernel<true, false>, beam_cluster_kernel<false, true>};
+        static Once once[3];
+        if (once[which].first()) {
+            cudaError_t err = cudaFuncSetAttribute(kernels[which], cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+            if (err == cudaSuccess) err = cudaFuncSetAttribute(kernels[which], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (err != cudaSuccess) return fail(-100, "beam_select: %s", cudaGetErrorString(err));
+            once[which].done();
+        }
+        return launch("beam_select", kernels[which], dim3(R * C), dim3(BM_CLUSTER_THREADS), (size_t)smem, stream, dim3(C, 1, 1), logits, V, n,
+                      scores, start, units, groups, k, out, status);
+    }
     const BeamPlan p = beam_plan(n, V);
     double* part_s = (double*)scratch;
     float* part_m = (float*)(part_s + (size_t)n * p.splits);
     float* gmax = part_m + (size_t)n * p.splits;
-    beam_scan_kernel<<<dim3(p.splits, n), BM_SCAN_THREADS, 0, stream>>>(logits, V, p.groups, p.per, gmax, part_m, part_s);
+    const dim3 grid(p.splits, n);
+    if (small) beam_scan_kernel<false, true><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
+    else if (vec) beam_scan_kernel<true, false><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
+    else beam_scan_kernel<false, false><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
     int rc = check_launch("beam_select");
     if (rc != 0) return rc;
-    beam_pick_kernel<<<R, BM_PICK_THREADS, 0, stream>>>(logits, V, n, scores, start, p.groups, p.splits, gmax, part_m, part_s, k,
-                                                        out_s, out_row, out_tok, status);
+    if (small)
+        beam_pick_kernel<BM_SMALL_GROUP><<<R, BM_PICK_THREADS, 0, stream>>>(logits, V, n, scores, start, groups, p.splits, gmax, part_m, part_s, k, out, status);
+    else
+        beam_pick_kernel<BM_GROUP><<<R, BM_PICK_THREADS, 0, stream>>>(logits, V, n, scores, start, groups, p.splits, gmax, part_m, part_s, k, out, status);
     return check_launch("beam_select_pick");
 }

@@ -16,6 +16,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace fd {
 
 // status bits written by kernels (host: flashdecode_cuda_b200/kernels.py)
@@ -182,6 +184,19 @@ constexpr int PDL_MIN_ROWS = 129;
 int add_rmsnorm(const void* delta, int delta_dtype, int n_parts, long long part_stride, float* resid, int write_resid,
                 const void* weight, int w_dtype, float eps, void* out, int out_dtype, const int* rows, int n_out, int H,
                 float dscale, bool pdl, cudaStream_t stream);
+}  // namespace fd
+
+namespace fd {
+// A kernel's attributes are set once per device (a microsecond of the host's time each).
+struct Once {
+    std::atomic<unsigned long long> devices{0};
+    static unsigned long long mine() {
+        int dev = 0;
+        return cudaGetDevice(&dev) == cudaSuccess && dev < 64 ? 1ull << dev : 0ull;
+    }
+    bool first() const { return (devices.load(std::memory_order_relaxed) & mine()) == 0; }
+    void done() { devices.fetch_or(mine(), std::memory_order_relaxed); }
+};
 }  // namespace fd
 
 #define FD_REQUIRE(cond, code, ...) \

@@ -125,21 +125,23 @@ extern "C" int fd_copy_blocks(void* pool, int planes, long long num_blocks, int 
     return check_launch("copy_blocks");
 }
 
-// states: n_states addresses; bytes: of one slot of each; src, dst [n] int (device).
+// states: n_states addresses; bytes: of all slots of each; src, dst [n] int (device).
 extern "C" int fd_copy_states(void* const* states, const long long* bytes, int n_states, int slots, const int* src, const int* dst,
                               int n, int* status, cudaStream_t stream) {
     if (n == 0 || n_states == 0) return 0;
+    if (slots == 0) return 0;
     FD_REQUIRE(n > 0 && n <= 65535 && n_states > 0 && slots > 0, -2, "copy_states: %d copies of %d states of %d slots", n, n_states, slots);
     for (int at = 0; at < n_states; at += CP_STATES) {
         StateList L;
         L.n = 0;
         long long chunks = 0;
         for (int j = at; j < n_states && j < at + CP_STATES; ++j) {
-            if (bytes[j] <= 0) continue;
+            const long long one = bytes[j] / slots;
+            if (one <= 0) continue;
             L.base[L.n] = (unsigned char*)states[j];
-            L.bytes[L.n] = bytes[j];
+            L.bytes[L.n] = one;
             L.first[L.n++] = (int)chunks;
-            chunks += (bytes[j] + CP_CHUNK - 1) / CP_CHUNK;
+            chunks += (one + CP_CHUNK - 1) / CP_CHUNK;
             FD_REQUIRE(chunks < (1ll << 31), -2, "copy_states: states of too many bytes");
         }
         if (L.n == 0) continue;

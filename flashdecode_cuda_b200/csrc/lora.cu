@@ -185,8 +185,12 @@ static int launch_general(const LoraArgs& p, cudaStream_t stream) {
     const size_t smem = sizeof(float) * (LR_ROWS * LR_CHUNK + 2 * (size_t)LR_ROWS * W);
     const long long tiles = lora_max_tiles(p, LR_ROWS);
     FD_REQUIRE(tiles * C < (1ll << 31), -2, "lora_add: %d tokens", p.T);
-    const cudaError_t err = cudaFuncSetAttribute(lora_general_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
+    static Once once;
+    if (once.first()) {
+        const cudaError_t err = cudaFuncSetAttribute(lora_general_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
+        once.done();
+    }
     return launch("lora_add", lora_general_kernel<T>, dim3((unsigned)(tiles * C)), dim3(LR_THREADS), smem, stream, dim3(C, 1, 1), p);
 }
 

@@ -352,9 +352,13 @@ int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream) {
     FD_REQUIRE(tiles * C * copies < (1ll << 31), -2, "lora_add: %d tokens", p.T);
     const int W = p.S * p.R;
     const size_t smem = sizeof(float) * (LM_WARPS * LM_ROWS * LM_RED + (size_t)LM_ROWS * W) + 2 * sizeof(__nv_bfloat16) * (size_t)LM_ROWS * lora_row_places(p.S, p.R);
-    cudaError_t err = cudaFuncSetAttribute(lora_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
-    if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
+    static Once once;
+    if (once.first()) {
+        cudaError_t err = cudaFuncSetAttribute(lora_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+        if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
+        once.done();
+    }
     return launch("lora_add", lora_rows_kernel, dim3((unsigned)(tiles * C * copies)), dim3(LM_THREADS), smem, stream, dim3(C, 1, 1), p, copies);
 }
 

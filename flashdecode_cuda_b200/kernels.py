@@ -156,6 +156,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "fd_dense_decode": [P, P, I],
         "fd_sample": [P, I, I, P, P, P, c_ulonglong, P, P, P, P],
         "fd_beam_select": [P, I, I, P, P, I, I, P, P, P, P, P, P],
+        "fd_beam_select_set_form": [I],
         "fd_copy_blocks": [P, I, LL, I, I, LL, P, P, P, I, P, P],
         "fd_copy_states": [P, P, I, I, P, P, I, P, P],
         "fd_lora_add": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, P],
@@ -1626,25 +1627,42 @@ BEAM_MAX_ROWS, BEAM_MAX_CANDIDATES = 64, 128
 LORA_MAX_SLICES, LORA_MAX_RANK, LORA_MAX_PACKED = 4, 256, 512
 
 
-def _here(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    """All on the device that is current: the launch goes to its stream."""
-    d = first.device
-    if d.type != "cuda":
-        raise KernelError("kernels take CUDA tensors only; there is no CPU path")
-    if d.index != torch.cuda.current_device():
-        raise KernelError(f"the tensors are on {d}, but cuda:{torch.cuda.current_device()} is the current device")
-    for t in others:
-        if t is not None and t.device != d:
-            raise KernelError(f"tensors on {d} and on {t.device} in one call")
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise KernelError(what)
+def _pointers(*tensors: Optional[torch.Tensor]) -> list:
+    """The tensors' addresses (None for None): contiguous CUDA tensors on the device that is current, whose stream the launch
+    goes to.  (A call of these operators takes a few microseconds on the device, so what its checks cost on the host shows: the
+    index of a tensor's device is an integer, its ``device`` an object that costs three times as much.)"""
+    here, out = _current_device(), []
+    for t in tensors:
+        if t is None:
+            out.append(None)
+            continue
+        if t.get_device() != here:
+            if not t.is_cuda:
+                raise KernelError("kernels take CUDA tensors only; there is no CPU path")
+            raise KernelError(f"a tensor is on {t.device}, but cuda:{here} is the current device")
+        if not t.is_contiguous():
+            raise KernelError("kernels take contiguous tensors")
+        out.append(t.data_ptr())
+    return out
+
+
+def _here_stream() -> int:
+    return _raw_stream(_current_device()) if _raw_stream is not None else _stream()
 
 
 def beam_select_scratch_bytes(n: int, V: int) -> int:
-    return int(lib().fd_beam_select_scratch_bytes(n, V))
+    """Enough for any cut of the rows: 4 bytes per group of 128 logits (of 32, up to 16,384 of them), 12 per 32 units of 128."""
+    units = -(-V // 128)
+    return n * ((16 if V <= 16384 else 4) * units + 12 * (units // 32 + 1))
+
+
+def beam_select_set_form(form: int) -> None:
+    """Which form ``beam_select`` takes from now on: 1 = a thread-block cluster per request, in one launch; 2 = a kernel that streams all
+    rows and one that picks; 0 = by the sizes.  For tests and measurements."""
+    lib().fd_beam_select_set_form(int(form))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, row_start: torch.Tensor, out_scores: torch.Tensor,
@@ -1658,21 +1676,26 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, row_start: torch.Ten
     -inf is no candidate; a row whose score or normaliser is no finite number (a NaN or +inf among its logits, nothing but -inf) has
     none.  Places that no candidate fills: -inf, -1, -1.  ``scratch``: uint8 of ``beam_select_scratch_bytes(n, V)`` that the call may
     use; when omitted it is allocated."""
-    _need(logits.dim() == 2 and logits.dtype == torch.float32 and scores.dtype == torch.float32, "beam_select: logits [n, V] and scores are float32")
+    f32, i32 = torch.float32, torch.int32
+    if not (logits.dim() == 2 and logits.dtype is f32 and scores.dtype is f32):
+        raise KernelError("beam_select: logits [n, V] and scores are float32")
     n, V = logits.shape
-    R, k = out_scores.shape
-    _need(scores.shape == (n,), f"beam_select: {n} rows of logits, scores {tuple(scores.shape)}")
-    _need(row_start.dtype == torch.int32 and row_start.shape == (R + 1,), f"beam_select: row_start is int32 [{R + 1}]")
-    _need(out_rows.shape == (R, k) and out_tokens.shape == (R, k) and out_scores.dtype == torch.float32
-          and out_rows.dtype == out_tokens.dtype == torch.int32, "beam_select: outputs are float32, int32 and int32, all [R, k]")
-    _here(logits, scores, row_start, out_scores, out_rows, out_tokens, scratch, status)
-    need = lib().fd_beam_select_scratch_bytes(n, V)
+    wide = out_scores.shape
+    if not (len(wide) == 2 and out_rows.shape == wide and out_tokens.shape == wide and out_scores.dtype is f32 and out_rows.dtype is i32 and out_tokens.dtype is i32):
+        raise KernelError("beam_select: outputs are float32, int32 and int32, all [R, k]")
+    R, k = wide
+    if not (scores.numel() == n):
+        raise KernelError(f"beam_select: {n} rows of logits, {scores.numel()} scores")
+    if not (row_start.dtype is i32 and row_start.numel() == R + 1):
+        raise KernelError(f"beam_select: row_start is int32 [{R + 1}]")
+    need = beam_select_scratch_bytes(n, V)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    _need(scratch.dtype == torch.uint8 and scratch.numel() >= need and scratch.data_ptr() % 8 == 0,
-          f"beam_select: scratch is uint8, {need} of them, 8-byte aligned")
-    _check(lib().fd_beam_select(_ptr(logits), n, V, _ptr(scores), _ptr(row_start), R, k, _ptr(out_scores), _ptr(out_rows),
-                                _ptr(out_tokens), _ptr(scratch), _ptr(status), _stream()))
+    else:
+        if not (scratch.dtype is torch.uint8 and scratch.numel() >= need and scratch.data_ptr() % 8 == 0):
+            raise KernelError(f"beam_select: scratch is uint8, {need} of them, 8-byte aligned")
+    x, s, start, os, orow, ot, work, st = _pointers(logits, scores, row_start, out_scores, out_rows, out_tokens, scratch, status)
+    _check(lib().fd_beam_select(x, n, V, s, start, R, k, os, orow, ot, work, st, _here_stream()))
 
 
 def copy_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, count: torch.Tensor,
@@ -1680,34 +1703,35 @@ def copy_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, count:
     """pool[p, dst[i], :, :count[i]] = pool[p, src[i], :, :count[i]] for every plane p and copy i: the first ``count[i]`` tokens of a
     cache block.  ``pool`` [planes, blocks, heads, block_size, ...] of any type; ``src``, ``dst``, ``count`` int32 [n].  No block may
     be named twice in ``dst``, or in both ``src`` and ``dst``.  A block or count outside the pool is skipped and reported."""
-    _need(pool.dim() >= 4, "copy_blocks: the pool is [planes, blocks, heads, block_size, ...]")
-    planes, blocks, heads, size = pool.shape[:4]
+    shape, i32 = pool.shape, torch.int32
+    if not (len(shape) >= 4):
+        raise KernelError("copy_blocks: the pool is [planes, blocks, heads, block_size, ...]")
     n = src.numel()
-    _need(src.dtype == dst.dtype == count.dtype == torch.int32 and dst.numel() == n == count.numel(), f"copy_blocks: src, dst and count are int32 [{n}]")
-    _here(pool, src, dst, count, status)
+    if not (src.dtype is i32 and dst.dtype is i32 and count.dtype is i32 and dst.numel() == n == count.numel()):
+        raise KernelError(f"copy_blocks: src, dst and count are int32 [{n}]")
+    at, s, d, c, st = _pointers(pool, src, dst, count, status)
+    planes, blocks, heads, size = shape[:4]
     if pool.numel() == 0:
         return
-    row = pool.numel() // (planes * blocks * heads * size) * pool.element_size()
-    _check(lib().fd_copy_blocks(_ptr(pool), planes, blocks, heads, size, row, _ptr(src), _ptr(dst), _ptr(count), n, _ptr(status),
-                                _stream()))
+    _check(lib().fd_copy_blocks(at, planes, blocks, heads, size, pool.nbytes // (planes * blocks * heads * size), s, d, c, n, st, _here_stream()))
 
 
 def copy_states(states: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, status: Optional[torch.Tensor] = None) -> None:
     """state[dst[i]] = state[src[i]] for every tensor [slots, ...] of ``states`` and copy i.  ``src``, ``dst`` int32 [n]; no slot may be
     named twice in ``dst``, or in both.  A slot that does not exist is skipped and reported."""
-    n = src.numel()
-    _need(src.dtype == dst.dtype == torch.int32 and dst.numel() == n, f"copy_states: src and dst are int32 [{n}]")
-    if not states:
+    n, i32 = src.numel(), torch.int32
+    if not (src.dtype is i32 and dst.dtype is i32 and dst.numel() == n):
+        raise KernelError(f"copy_states: src and dst are int32 [{n}]")
+    s, d, st, *at = _pointers(src, dst, status, *states)
+    m = len(at)
+    if m == 0:
         return
-    slots = states[0].shape[0]
-    _here(src, dst, status, *states)
-    if slots == 0:
-        return
+    slots = states[0].size(0) if states[0].dim() else -1
     for t in states:
-        _need(t.shape[0] == slots, f"copy_states: states of {slots} and of {t.shape[0]} slots")
-    m = len(states)
-    at, size = (c_void_p * m)(*map(_ptr, states)), (c_longlong * m)(*[t.nbytes // slots for t in states])
-    _check(lib().fd_copy_states(at, size, m, slots, _ptr(src), _ptr(dst), n, _ptr(status), _stream()))
+        if not t.dim() or t.size(0) != slots:
+            raise KernelError("copy_states: the states are [slots, ...], all of one number of slots")
+    sizes = [t.nbytes for t in states]
+    _check(lib().fd_copy_states((c_void_p * m)(*at), (c_longlong * m)(*sizes), m, slots, s, d, n, st, _here_stream()))
 
 
 def lora_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, ranks: torch.Tensor, order: torch.Tensor,
@@ -1728,15 +1752,18 @@ def lora_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Ten
     out = y if out is None else out
     T, Kd = x.shape
     E, N, R = b.shape
-    _need(x.dtype == a.dtype == b.dtype == y.dtype == out.dtype, "lora_add: x, a, b, y and out are of one type")
-    _need(a.shape == (E, slices * R, Kd), f"lora_add: a is [{E}, {slices * R}, {Kd}], not {tuple(a.shape)}")
-    _need(y.shape == (T, N) and out.shape == (T, N), f"lora_add: y and out are [{T}, {N}]")
-    _need(scale.dtype == torch.float32 and scale.shape == (E,) and ranks.dtype == torch.int32 and ranks.shape == (E,),
-          f"lora_add: scale is float32 [{E}], ranks int32 [{E}]")
-    n_seg = ids.numel()
-    _need(order.dtype == start.dtype == ids.dtype == torch.int32 and order.shape == (T,) and start.shape == (n_seg + 1,),
-          f"lora_add: order, start and ids are int32 [{T}], [{n_seg + 1}], [{n_seg}]")
-    _need(col_slice is None or (col_slice.dtype == torch.uint8 and col_slice.numel() * 8 == N), "lora_add: col_slice is uint8 [N / 8]")
-    _here(x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status)
-    _check(lib().fd_lora_add(_ptr(x), _ptr(a), _ptr(b), _ptr(scale), _ptr(ranks), _ptr(order), _ptr(start), _ptr(ids), _ptr(y),
-                             _ptr(out), _ptr(col_slice), _dt(x.dtype), T, Kd, N, E, R, slices, n_seg, _ptr(status), _stream()))
+    dt, i32, n_seg = x.dtype, torch.int32, ids.numel()
+    if not (a.dtype is dt and b.dtype is dt and y.dtype is dt and out.dtype is dt):
+        raise KernelError("lora_add: x, a, b, y and out are of one type")
+    if not (a.shape == (E, slices * R, Kd)):
+        raise KernelError(f"lora_add: a is [{E}, {slices * R}, {Kd}], not {tuple(a.shape)}")
+    if not (y.shape == (T, N) and (out is y or out.shape == (T, N))):
+        raise KernelError(f"lora_add: y and out are [{T}, {N}]")
+    if not (scale.dtype is torch.float32 and scale.numel() == E and ranks.dtype is i32 and ranks.numel() == E):
+        raise KernelError(f"lora_add: scale is float32 [{E}], ranks int32 [{E}]")
+    if not (order.dtype is i32 and start.dtype is i32 and ids.dtype is i32 and order.numel() == T and start.numel() == n_seg + 1):
+        raise KernelError(f"lora_add: order, start and ids are int32 [{T}], [{n_seg + 1}], [{n_seg}]")
+    if not (col_slice is None or (col_slice.dtype is torch.uint8 and col_slice.numel() * 8 == N)):
+        raise KernelError("lora_add: col_slice is uint8 [N / 8]")
+    _check(lib().fd_lora_add(*_pointers(x, a, b, scale, ranks, order, start, ids, y, out, col_slice), _dt(dt), T, Kd, N, E, R, slices,
+                             n_seg, _ptr(status), _here_stream()))

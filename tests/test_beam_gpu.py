@@ -244,3 +244,22 @@ def test_refusals():
         K.copy_states([f(3, 4).t()], i(1), i(1))
     with pytest.raises(K.KernelError):
         K.copy_states([f(3, 4).cpu()], i(1), i(1))
+
+
+@pytest.mark.parametrize("form", [1, 2])
+@pytest.mark.parametrize("V,beams,k", [(1, [3], 4), (130, [2, 0, 64, 1], 128), (4096, [4, 4], 8), (50257, [1, 8, 3], 16), (151936, [4], 8), (700, [1] * 150, 3)])
+def test_both_forms(form, V, beams, k):
+    K.beam_select_set_form(form)
+    try:
+        g = torch.Generator().manual_seed(V * 3 + k)
+        start = [0]
+        for b in beams:
+            start.append(start[-1] + b)
+        n = start[-1]
+        x = 3.0 * torch.randn(n, V, generator=g)
+        x[:, V // 2] = -math.inf
+        check(x, -20.0 * torch.rand(n, generator=g), start, k)
+        x.zero_()                                        # constant rows: the exact cuts
+        check(x, torch.zeros(n), start, k)
+    finally:
+        K.beam_select_set_form(0)
