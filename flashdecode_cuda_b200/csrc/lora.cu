@@ -200,6 +200,17 @@ using namespace fd;
 
 extern "C" int fd_sm_count();
 
+// Tokens per segment, on average, from which tiles of 128 are taken.
+constexpr int LORA_TILE_TOKENS = 32;
+
+static int g_lora_form = 0;
+// Which form the bfloat16 steps on the tensor cores take from now on: 1 = tiles of 16 tokens, 2 = tiles of 128 where they take the
+// sizes, 0 = by the sizes.  For tests and measurements.
+extern "C" int fd_lora_set_form(int form) {
+    g_lora_form = form;
+    return 0;
+}
+
 extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const float* scale, const int* ranks, const int* order,
                            const int* start, const int* ids, const void* y, void* out, const unsigned char* col_slice, int dtype,
                            int T, int K, int N, int E, int R, int S, int n_seg, int* status, cudaStream_t stream) {
@@ -211,5 +222,8 @@ extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const fl
     FD_REQUIRE(S == 1 || (col_slice != nullptr && N % 8 == 0), -2, "lora_add: %d packed projections need col_slice and N a multiple of 8", S);
     const LoraArgs p{x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status, T, K, N, E, R, S, n_seg};
     if (dtype == 0) return launch_general<float>(p, stream);
-    return lora_mma_takes(p) ? lora_rows(p, fd_sm_count(), stream) : launch_general<__nv_bfloat16>(p, stream);
+    if (!lora_mma_takes(p)) return launch_general<__nv_bfloat16>(p, stream);
+    // (the adapters' tokens are known on the device only: by their average)
+    const bool many = g_lora_form == 0 ? T >= LORA_TILE_TOKENS * n_seg : g_lora_form == 2;
+    return many && lora_tiles_take(p) ? lora_tiles(p, fd_sm_count(), stream) : lora_rows(p, fd_sm_count(), stream);
 }

@@ -75,5 +75,8 @@ inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (long long
 // The kernels on the tensor cores (lora_mma.cu): whether they take the sizes, and the launch.
 bool lora_mma_takes(const LoraArgs& p);
 int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream);
+// ... and with tiles of 128 tokens (lora_tcgen05.cu): whether they take the sizes too, and the launch.
+bool lora_tiles_take(const LoraArgs& p);
+int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream);
 
 }  // namespace fd

@@ -157,6 +157,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "fd_sample": [P, I, I, P, P, P, c_ulonglong, P, P, P, P],
         "fd_beam_select": [P, I, I, P, P, I, I, P, P, P, P, P, P],
         "fd_beam_select_set_form": [I],
+        "fd_lora_set_form": [I],
         "fd_copy_blocks": [P, I, LL, I, I, LL, P, P, P, I, P, P],
         "fd_copy_states": [P, P, I, I, P, P, I, P, P],
         "fd_lora_add": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, P],
@@ -1732,6 +1733,12 @@ def copy_states(states: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Te
             raise KernelError("copy_states: the states are [slots, ...], all of one number of slots")
     sizes = [t.nbytes for t in states]
     _check(lib().fd_copy_states((c_void_p * m)(*at), (c_longlong * m)(*sizes), m, slots, s, d, n, st, _here_stream()))
+
+
+def lora_set_form(form: int) -> None:
+    """Which form ``lora_add`` takes from now on for bfloat16 tensors of 16-byte pieces: 1 = tiles of 16 tokens of one adapter, 2 = tiles
+    of 128 (where they take the sizes), 0 = by the number of tokens per adapter.  For tests and measurements."""
+    lib().fd_lora_set_form(int(form))
 
 
 def lora_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, ranks: torch.Tensor, order: torch.Tensor,

@@ -259,3 +259,18 @@ def test_refusals():
                 dict(slices=4, a=f(2, 4 * 136, 16), b=f(2, 24, 136), col_slice=torch.zeros(3, dtype=torch.uint8, device=DEV))):
         with pytest.raises(K.KernelError):
             K.lora_add(**{**ok, **bad})
+
+
+@pytest.mark.parametrize("form", [1, 2])
+@pytest.mark.parametrize("T,Kd,N,E,R,S,tiled", [
+    (1, 64, 64, 1, 16, 1, False), (128, 64, 128, 1, 16, 1, False), (130, 72, 136, 1, 8, 1, False), (300, 1000, 264, 3, 24, 1, False),
+    (129, 4096, 1024, 2, 64, 1, False), (257, 640, 520, 2, 128, 1, False), (140, 328, 384, 2, 16, 3, False), (260, 512, 648, 3, 64, 3, False),
+    (135, 704, 512, 2, 40, 2, True), (270, 128, 136, 2, 96, 2, True), (20, 2048, 4096, 5, 32, 2, True), (900, 256, 1288, 4, 16, 4, True),
+    (129, 8, 8, 1, 8, 1, False)])
+def test_both_forms(form, T, Kd, N, E, R, S, tiled):
+    K.lora_set_form(form)
+    try:
+        check("bfloat16", T, Kd, N, E, R, S, tiled)
+        check("bfloat16", T, Kd, N, E, R, S, tiled, token=[(i // 150) % E for i in range(T)], in_place=True, seed=3)
+    finally:
+        K.lora_set_form(0)
