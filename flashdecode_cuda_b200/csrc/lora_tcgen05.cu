@@ -3,14 +3,14 @@
 // Such a step reads x and y and writes out, and does 2 r operations with every element of them, so it is bound by memory as long
 // as the products keep up: at rank 64 they would take all that mma.sync has, which is why they are tcgen05.mma here.  A cluster of CTAs
 // takes 128 tokens of one adapter:
-//   1. D1 [128 x S r] = x A^T over the CTA's share of K.  Blocks of 64 columns of x (rows by the tokens' list, so they may lie
-//      anywhere) and of A go to a ring of swizzled tiles by cp.async; one thread issues the MMAs; D1 is in tensor memory.
+//   1. D1 [128 x S r] = x A^T over the CTA's share of K, in tensor memory.  Blocks of 64 columns of x and A go through a ring of
+//      swizzled tiles.
 //   2. The cluster's partial sums are added in the order of the ranks: each CTA adds 128 / C tokens' and hands them to all,
 //      as two bfloat16 numbers each (what rounding takes away from the first is the second: 2^-17 of A x is lost, not 2^-9).
-//   3. D2 [128 x 128] = h B^T for the CTA's share of the columns.  y and B of the next tile are on their way while this one is
-//      multiplied and stored.  A tile whose columns belong to several slices (gate and up) multiplies each slice's h with the rows
-//      of B that are its own, the others zero.
-// y comes to and out leaves from shared memory in rows, so that both move whole lines although a thread's D2 is one row.
+//   3. D2 [128 x 128] = h B^T for the CTA's share of the columns, a product for every slice that has columns in the tile (gate and up
+//      both); the epilogue takes each column from its own.  The tiles' y and B are a stage or two ahead.
+// One warp asks for copies, one thread issues MMAs, eight warps do the rest.  out takes y's place in shared memory, so that it leaves in
+// whole lines although a thread's share of D2 is a row.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -23,33 +23,31 @@ namespace fd {
 
 namespace cg = cooperative_groups;
 
-constexpr int LT_ROWS = 128, LT_COLS = 128, LT_THREADS = 256;
-constexpr int LT_X_BYTES = LT_ROWS * 128;        // a block of 64 columns of x: rows of 128 bytes
-constexpr int LT_TILE = 128 * 128;               // a tile of 64 columns of 128 rows
-constexpr int LT_Y_ROW = LT_COLS * 2 + 16;       // a row of y in shared memory; 16: neighbouring rows in other banks
-constexpr int LT_Y_BYTES = LT_ROWS * LT_Y_ROW;
-constexpr int LT_STAGES = 8;
-constexpr int LT_SMEM = 222 * 1024;
+constexpr int LT_ROWS = 128, LT_COLS = 128;
+constexpr int LT_EPI = 8, LT_THREADS = (2 + LT_EPI) * 32;
+constexpr int LT_TILE = 128 * 128;               // bytes of a tile of 64 columns of 128 rows
+constexpr int LT_Y_BYTES = 2 * LT_TILE;          // y's tile of 128 columns: two of those
+constexpr int LT_RING = 8, LT_OUT_RING = 3;      // most stages of step 1 and of step 3
+constexpr int LT_SMEM = 225 * 1024;
 constexpr int LT_MAX_W = 192;                    // columns of D1
 
 struct LoraTilePlan {
     int chunks;              // 64-column tiles of a slice of h
-    int stages;              // of the ring of step 1
+    int stages, out_stages;  // of the rings of steps 1 and 3
     size_t smem;
 };
 
 static LoraTilePlan lora_tile_plan(const LoraArgs& p) {
     LoraTilePlan f;
-    const int r16 = (p.R + 15) / 16 * 16, W = p.S * r16;
+    const int W = p.S * ((p.R + 15) / 16 * 16);
     f.chunks = (p.R + 63) / 64;
-    const size_t stage = LT_X_BYTES + (size_t)W * 128;
-    const size_t later = (size_t)p.S * f.chunks * LT_TILE * 3 + 2 * LT_Y_BYTES;          // hi, lo, B; y twice
-    f.stages = (int)std::min<size_t>(LT_STAGES, (LT_SMEM - 1024) / stage);
-    f.smem = 1024 + std::max(later, f.stages * stage);
-    // the partial sums lie behind hi and lo
-    const size_t sums = (size_t)p.S * f.chunks * LT_TILE * 2 + (size_t)LT_ROWS * (W + 4) * 4;
-    f.smem = std::max(f.smem, 1024 + sums);
-    if (W > LT_MAX_W || f.stages < 4 || f.smem > LT_SMEM) f.stages = 0;
+    const size_t room = LT_SMEM - 1024, h = 2 * (size_t)p.S * f.chunks * LT_TILE;         // h: both numbers
+    const size_t stage = LT_TILE + (size_t)W * 128, out_stage = LT_Y_BYTES + (size_t)f.chunks * LT_TILE;
+    const size_t sums = h + (size_t)LT_ROWS * (W + 4) * 4;                                  // step 2's sums lie behind h
+    f.stages = (int)std::min<size_t>(LT_RING, room / stage);
+    f.out_stages = h < room ? (int)std::min<size_t>(LT_OUT_RING, (room - h) / out_stage) : 0;
+    f.smem = 1024 + std::max(std::max(f.stages * stage, h + f.out_stages * out_stage), sums);
+    if (W > LT_MAX_W || f.stages < 3 || f.out_stages < 2 || f.smem > LT_SMEM) f.stages = 0;
     return f;
 }
 
@@ -57,11 +55,65 @@ bool lora_tiles_take(const LoraArgs& p) { return lora_tile_plan(p).stages > 0; }
 
 __device__ __forceinline__ uint32_t lt_swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
+// four rows of a map with boxes of one row
+__device__ __forceinline__ void lt_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int r0, int r1, int r2, int r3) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+__device__ __forceinline__ void lt_ld8(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+}
+
+// x and y in boxes of 128 rows, of 16, and of one (for gathers).
+struct LoraMaps {
+    CUtensorMap x[3], y[3], a, b;
+};
+
+// The rows of a tile's tokens: neighbours all of them (a prompt's tokens are), or 16 by 16, or gathered four by four, which the copy
+// engine does some ten times slower.
+struct LoraRows {
+    bool all;
+    int first;               // of the tile
+    int group;               // lanes 0 .. 7: the first of 16 neighbours, or -1
+    int rows[4];             // this lane's four of the tile
+    // rows of no token read others', and what comes of them is not stored
+    __device__ __forceinline__ explicit LoraRows(const int* tok, int count) {
+        const int lane = threadIdx.x & 31;
+        first = max(tok[0], 0);
+        bool row = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = tok[lane * 4 + i];
+            rows[i] = max(t, 0);
+            row = row && (lane * 4 + i >= count || t == tok[0] + lane * 4 + i);
+        }
+        all = __all_sync(0xffffffffu, row && tok[0] >= 0);
+        const int g = (lane & 7) * 16;
+        group = max(tok[g], 0);
+        for (int i = 1; i < 16; ++i)
+            if (g + i < count && tok[g + i] != group + i) group = -1;
+        if (tok[g] < 0 && g < count) group = -1;
+    }
+    // the 64 columns from col on of all rows, to the tile at dst; called by a whole warp
+    __device__ __forceinline__ void ask(uint32_t dst, const CUtensorMap* maps, uint32_t bar, int col) const {
+        const int lane = threadIdx.x & 31;
+        if (all) {
+            if (lane == 0) tma_load_2d(dst, maps, bar, col, first);
+            return;
+        }
+        if (lane < 8 && group >= 0) tma_load_2d(dst + lane * 2048, maps + 1, bar, col, group);
+        if (__shfl_sync(0xffffffffu, group, lane >> 2) < 0) lt_gather4(dst + lane * 512, maps + 2, bar, col, rows[0], rows[1], rows[2], rows[3]);
+    }
+};
+
 __global__ void __launch_bounds__(LT_THREADS, 1)
-lora_tile_kernel(const LoraArgs p, const int chunks, const int stages, const unsigned long long wait_ns) {
+lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const int chunks, const int stages, const int out_stages,
+                 const unsigned long long wait_ns) {
     extern __shared__ unsigned char lt_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)lt_smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long bars[LT_STAGES + 1];      // the MMAs that read a stage are done; D2 (and, at first, D1) is
+    __shared__ __align__(8) unsigned long long full[LT_RING], empty[LT_RING], out_full[LT_OUT_RING], out_empty[LT_OUT_RING], acc_full[2],
+        acc_empty[2], d1_full;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ int tok[LT_ROWS];
@@ -70,7 +122,19 @@ lora_tile_kernel(const LoraArgs p, const int chunks, const int stages, const uns
     const int C = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         abort_flag = 0;
-        for (int i = 0; i <= LT_STAGES; ++i) mbar_init(s_addr(&bars[i]), 1);
+        for (int i = 0; i < LT_RING; ++i) {
+            mbar_init(s_addr(&full[i]), 1);
+            mbar_init(s_addr(&empty[i]), 1);
+        }
+        for (int i = 0; i < LT_OUT_RING; ++i) {
+            mbar_init(s_addr(&out_full[i]), 1);
+            mbar_init(s_addr(&out_empty[i]), LT_EPI);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_addr(&acc_full[i]), 1);
+            mbar_init(s_addr(&acc_empty[i]), LT_EPI);
+        }
+        mbar_init(s_addr(&d1_full), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -85,10 +149,10 @@ lora_tile_kernel(const LoraArgs p, const int chunks, const int stages, const uns
     __syncthreads();
     const LoraTile tile = tile_s;
     if (tile.adapter == -2) return;                              // the same for the whole cluster
-    const __nv_bfloat16* y = static_cast<const __nv_bfloat16*>(p.y);
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
     const int e = max(tile.adapter, 0), r = tile.adapter < 0 ? 0 : min(max(p.ranks[e], 0), p.R);
     if (r == 0) {                                                // nothing to add
+        const __nv_bfloat16* y = static_cast<const __nv_bfloat16*>(p.y);
         if (static_cast<const void*>(out) == p.y) return;
         for (int i = warp; i < tile.count; i += LT_THREADS / 32)
             if (tok[i] >= 0)
@@ -96,110 +160,94 @@ lora_tile_kernel(const LoraArgs p, const int chunks, const int stages, const uns
                     *reinterpret_cast<uint4*>(out + (size_t)tok[i] * p.N + n) = *reinterpret_cast<const uint4*>(y + (size_t)tok[i] * p.N + n);
         return;
     }
-    if (warp == 0) {
+    if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t d1 = tmem_slot, d2 = d1 + 256;
-    const uint32_t base = s_addr(smem);
-    const int r16 = (r + 15) / 16 * 16, W = p.S * r16;           // D1's columns: each slice's in whole MMAs
-    const uint32_t done = s_addr(&bars[LT_STAGES]);
+    const uint32_t tmem = tmem_slot, base = s_addr(smem);
+    // D1's columns: R of each slice, in whole MMAs.  (Those behind an adapter's rank are dropped: a slice's rows of A come in one copy,
+    // whose size is the same for every adapter, and it is copies that cost, some 85 cycles of the asking warp each.)
+    const int r16 = (p.R + 15) / 16 * 16, W = p.S * r16;
+    const int hbytes = p.S * chunks * LT_TILE;                   // hi, then lo, as tiles [slice][64 columns] of 128 rows
+    const int blocks = (p.K + 63) / 64, bper = (blocks + C - 1) / C, b0 = rank * bper, nb = max(0, min(blocks, b0 + bper) - b0);
+    const int stage_bytes = LT_TILE + W * 128, out_stage_bytes = LT_Y_BYTES + chunks * LT_TILE;
+    const int tiles = (p.N + LT_COLS - 1) / LT_COLS;
+    const int accs = p.S <= 2 ? 2 : 1;                           // accumulators of step 3: S x 128 of the 512 columns each
 
     // ---- 1. D1 = x A^T over this CTA's share of K ----
-    const int blocks = (p.K + 63) / 64, bper = (blocks + C - 1) / C, b0 = rank * bper, nb = max(0, min(blocks, b0 + bper) - b0);
-    const int stage_bytes = LT_X_BYTES + W * 128;
-    {
-        const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x);
-        const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + (size_t)e * p.S * p.R * p.K;
-        const int chunk = tid & 7, row0 = tid >> 3;              // a thread's 16 bytes of rows row0, row0 + 32, ...
-        const __nv_bfloat16* xr[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) xr[i] = tok[row0 + 32 * i] >= 0 ? x + (size_t)tok[row0 + 32 * i] * p.K : nullptr;
-        auto fetch = [&](int it) {
-            const int k = (b0 + it) * 64 + chunk * 8;
-            const bool in = k < p.K;                             // K is a multiple of 8
-            const uint32_t s = base + (it % stages) * stage_bytes;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool there = in && xr[i] != nullptr;
-                cp_async16(s + lt_swizzled(row0 + 32 * i, chunk), there ? xr[i] + k : x, there ? 16 : 0);
-            }
-            for (int u = row0; u < W; u += 32) {
-                const int sl = u / r16, j = u - sl * r16;
-                const bool there = in && j < p.R;
-                cp_async16(s + LT_X_BYTES + lt_swizzled(u, chunk), there ? a + (size_t)(sl * p.R + j) * p.K + k : a, there ? 16 : 0);
-            }
-        };
-        // two stages of slack: the one that is filled again was multiplied two blocks ago
-        const int ahead = stages - 2;
-        for (int it = 0; it < ahead; ++it) {
-            if (it < nb) fetch(it);
-            cp_async_commit();
+    const LoraRows rows(tok, tile.count);
+    if (warp == 0) {
+        for (int it = 0; it < nb; ++it) {
+            const int s = it % stages, k = (b0 + it) * 64;
+            if (it >= stages && !__all_sync(0xffffffffu, mbar_wait(s_addr(&empty[s]), (it / stages - 1) & 1, &abort_flag, p.status, wait_ns))) break;
+            const uint32_t bar = s_addr(&full[s]), at = base + s * stage_bytes;
+            if (lane == 0) mbar_expect_tx(bar, stage_bytes);
+            __syncwarp();
+            if (rows.all && lane == 0) tma_load_2d(at, maps.x, bar, k, rows.first);
+            if (lane < p.S) tma_load_2d(at + LT_TILE + lane * r16 * 128, &maps.a, bar, k, (e * p.S + lane) * p.R);
         }
+    } else if (warp == 1 && lane == 0) {
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(W >> 3) << 17) | ((uint32_t)(LT_ROWS >> 4) << 24);
         for (int it = 0; it < nb; ++it) {
-            // blocks up to `it` have landed: the newest ahead - 1 groups may be under way
-            switch (ahead) {
-                case 2: cp_async_wait<1>(); break;
-                case 3: cp_async_wait<2>(); break;
-                case 4: cp_async_wait<3>(); break;
-                case 5: cp_async_wait<4>(); break;
-                default: cp_async_wait<5>(); break;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncthreads();
-            if (tid == 0 && !abort_flag) {
-                tc_fence_after();
-                const uint32_t s = base + (it % stages) * stage_bytes;
-                const uint64_t adesc = smem_desc_sw128(s), bdesc = smem_desc_sw128(s + LT_X_BYTES);
+            const int s = it % stages;
+            if (!mbar_wait(s_addr(&full[s]), (it / stages) & 1, &abort_flag, p.status, wait_ns)) break;
+            tc_fence_after();
+            const uint64_t adesc = smem_desc_sw128(base + s * stage_bytes), bdesc = smem_desc_sw128(base + s * stage_bytes + LT_TILE);
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) tc_mma(d1, adesc + 2 * kk, bdesc + 2 * kk, idesc, (it | kk) != 0);
-                tc_commit(s_addr(&bars[it % stages]));
-                if (it == nb - 1) tc_commit(done);
-            }
-            const int next = it + ahead;
-            if (next < nb) {
-                if (it >= 2) mbar_wait(s_addr(&bars[(it - 2) % stages]), ((it - 2) / stages) & 1, &abort_flag, p.status, wait_ns);
-                fetch(next);
-            }
-            cp_async_commit();
+            for (int kk = 0; kk < 4; ++kk) tc_mma(tmem, adesc + 2 * kk, bdesc + 2 * kk, idesc, (it | kk) != 0);
+            tc_commit(s_addr(&empty[s]));
         }
-        cp_async_wait<0>();
-        if (nb > 0) mbar_wait(done, 0, &abort_flag, p.status, wait_ns);
+        tc_commit(s_addr(&d1_full));
     }
-    uint32_t phase = nb > 0 ? 1 : 0;                             // of `done`
-    tc_fence_after();
-    __syncthreads();
+    else if (warp >= 2 && !rows.all) {
+        // rows that lie here and there take many copies: eight warps ask for 16 rows each
+        const int g = warp - 2, first = __shfl_sync(0xffffffffu, rows.group, g);
+        for (int it = 0; it < nb; ++it) {
+            const int s = it % stages, k = (b0 + it) * 64;
+            if (it >= stages && !__all_sync(0xffffffffu, mbar_wait(s_addr(&empty[s]), (it / stages - 1) & 1, &abort_flag, p.status, wait_ns))) break;
+            const uint32_t bar = s_addr(&full[s]), at = base + s * stage_bytes;
+            if (first >= 0) {
+                if (lane == 0) tma_load_2d(at + g * 2048, maps.x + 1, bar, k, first);
+            } else if (lane >> 2 == g) {
+                lt_gather4(at + lane * 512, maps.x + 2, bar, k, rows.rows[0], rows.rows[1], rows.rows[2], rows.rows[3]);
+            }
+            __syncwarp();
+        }
+    }
+    __syncwarp();
 
     // ---- 2. the cluster's sums ----
-    const int hbytes = p.S * chunks * LT_TILE;                   // hi, then lo, as tiles [slice][64 columns] of 128 rows
-    const int quarter = warp & 3, half = warp >> 2;              // a warp reads lanes 32 quarter .. of tensor memory
+    const int quarter = warp & 3, half = (warp - 2) >> 2, et = tid - 64;         // of the epilogue warps: the lanes of tensor memory, the columns
     float* part = reinterpret_cast<float*>(smem + 2 * hbytes);   // [128][W + 4]
-    {
+    if (warp >= 2) {
+        // (every copy and MMA of step 1 has ended then: the ring's memory is free)
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(s_addr(&d1_full), 0, &abort_flag, p.status, wait_ns)) && nb > 0;
+        tc_fence_after();
         const int row = quarter * 32 + lane;
         for (int c0 = half * 16; c0 < W; c0 += 32) {
             uint32_t v[16];
-            if (nb > 0) {
-                tc_ld16(d1 + ((uint32_t)(quarter * 32) << 16) + c0, v);
+            if (ok) {
+                tc_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
                 tc_wait_ld();
             }
             const int j0 = c0 % r16;                             // r16 is a multiple of 16: one slice
             float f[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = nb > 0 && j0 + i < r ? __uint_as_float(v[i]) : 0.f;
+            for (int i = 0; i < 16; ++i) f[i] = ok && j0 + i < r ? __uint_as_float(v[i]) : 0.f;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + row * (W + 4) + c0 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
         }
+        tc_fence_before();
     }
-    tc_fence_before();
+    __syncwarp();
     cluster.sync();
     {
-        const int rows = LT_ROWS / C, per_row = W / 8;
-        for (int i = tid; i < rows * per_row; i += LT_THREADS) {
-            const int row = rank * rows + i / per_row, c = (i % per_row) * 8, sl = c / r16, j = c - sl * r16;
+        const int share = LT_ROWS / C, per_row = W / 8;
+        for (int i = tid; i < share * per_row; i += LT_THREADS) {
+            const int row = rank * share + i / per_row, c = (i % per_row) * 8, sl = c / r16, j = c - sl * r16;
             float v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = 0.f;
@@ -219,125 +267,137 @@ lora_tile_kernel(const LoraArgs p, const int chunks, const int stages, const uns
             }
         }
     }
-    asm volatile("fence.proxy.async;" ::: "memory");             // written by threads, read by the MMAs of any CTA
+    asm volatile("fence.proxy.async;" ::: "memory");             // written by threads, read by the MMAs of any CTA; and part's memory takes copies
+    __syncwarp();
     cluster.sync();
     asm volatile("fence.proxy.async;" ::: "memory");
 
     // ---- 3. out = y + scale h B^T for this CTA's tiles of 128 columns ----
-    const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.b) + (size_t)e * p.N * p.R;
-    const float scale = p.scale[e];
-    const int tiles = (p.N + LT_COLS - 1) / LT_COLS;
-    const uint32_t bbuf = base + 2 * hbytes, ybuf = bbuf + hbytes;
-    unsigned char* ymem = smem + 3 * hbytes;
-    auto fetch_y = [&](int n0, int buf) {
-        const int chunk = tid & 15, n = n0 + chunk * 8;
-        if (n < p.N)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = (tid >> 4) + 16 * i;
-                if (tok[row] >= 0) cp_async16(ybuf + buf * LT_Y_BYTES + row * LT_Y_ROW + chunk * 16, y + (size_t)tok[row] * p.N + n, 16);
-            }
-    };
-    // the slices among the columns of a tile, as bits
-    auto slices_of = [&](int n0) -> unsigned {
-        if (p.col_slice == nullptr) return 1u;
-        const int n = n0 + (lane & 15) * 8;
-        return __reduce_or_sync(0xffffffffu, n < p.N ? 1u << min((int)__ldg(p.col_slice + n / 8), p.S - 1) : 0u);
-    };
-    auto fetch_b = [&](int n0, unsigned present) {
-        const int per_row = r16 / 8, row = tid >> 1, n = n0 + row;                     // two threads share a row
-        const int own = p.col_slice != nullptr && n < p.N ? min((int)__ldg(p.col_slice + n / 8), p.S - 1) : 0;
-        for (int sl = 0; sl < p.S; ++sl) {
-            if (!(present >> sl & 1)) continue;
-            const uint32_t at = bbuf + sl * chunks * LT_TILE;
-            for (int c = tid & 1; c < per_row; c += 2) {
-                const bool there = n < p.N && own == sl && c * 8 < p.R;
-                cp_async16(at + (c >> 3) * LT_TILE + lt_swizzled(row, c & 7), there ? b + (size_t)n * p.R + c * 8 : b, there ? 16 : 0);
-            }
+    const uint32_t ring = base + 2 * hbytes;                     // stages: y, then B
+    if (warp == 0) {
+        int i = 0;
+        for (int t = rank; t < tiles; t += C, ++i) {
+            const int s = i % out_stages, n0 = t * LT_COLS;
+            if (i >= out_stages && !__all_sync(0xffffffffu, mbar_wait(s_addr(&out_empty[s]), (i / out_stages - 1) & 1, &abort_flag, p.status, wait_ns))) break;
+            const uint32_t bar = s_addr(&out_full[s]), at = ring + s * out_stage_bytes;
+            const bool both = n0 + 64 < p.N;
+            if (lane == 0) mbar_expect_tx(bar, both ? out_stage_bytes : out_stage_bytes - LT_TILE);
+            __syncwarp();
+            rows.ask(at, maps.y, bar, n0);
+            if (both) rows.ask(at + LT_TILE, maps.y, bar, n0 + 64);
+            if (lane < chunks) tma_load_2d(at + LT_Y_BYTES + lane * LT_TILE, &maps.b, bar, lane * 64, e * p.N + n0);
         }
-    };
-    const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT_COLS >> 3) << 17) | ((uint32_t)(LT_ROWS >> 4) << 24);
-    int buf = 0;
-    unsigned present = 0;
-    if (rank < tiles) {
-        present = slices_of(rank * LT_COLS);
-        fetch_y(rank * LT_COLS, 0);
-        fetch_b(rank * LT_COLS, present);
-    }
-    cp_async_commit();
-    for (int t = rank; t < tiles; t += C) {
-        const int n0 = t * LT_COLS, n1 = (t + C) * LT_COLS;
-        cp_async_wait<0>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
-        if (tid == 0 && !abort_flag) {
+        // copies that nobody waited for (after a wait that gave up) end before their memory is given up
+        if (abort_flag) {
+            int here = 0;
+            for (int j = max(0, i - out_stages); j < i; ++j) mbar_wait(s_addr(&out_full[j % out_stages]), (j / out_stages) & 1, &here, nullptr, wait_ns);
+            for (int it = max(0, nb - stages); it < nb; ++it) mbar_wait(s_addr(&full[it % stages]), (it / stages) & 1, &here, nullptr, wait_ns);
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT_COLS >> 3) << 17) | ((uint32_t)(LT_ROWS >> 4) << 24);
+        const int steps = (r + 15) / 16;                         // as far as the adapter's rank reaches
+        int i = 0;
+        for (int t = rank; t < tiles; t += C, ++i) {
+            const int s = i % out_stages, acc = i % accs, n = t * LT_COLS + (lane & 15) * 8;
+            // the slices that have columns in this tile
+            const unsigned present = p.col_slice == nullptr ? 1u
+                : __reduce_or_sync(0xffffffffu, n < p.N ? 1u << min((int)__ldg(p.col_slice + n / 8), p.S - 1) : 0u);
+            if (!__all_sync(0xffffffffu, mbar_wait(s_addr(&out_full[s]), (i / out_stages) & 1, &abort_flag, p.status, wait_ns))) break;
+            if (i >= accs && !__all_sync(0xffffffffu, mbar_wait(s_addr(&acc_empty[acc]), (i / accs - 1) & 1, &abort_flag, p.status, wait_ns))) break;
             tc_fence_after();
-            uint32_t more = 0;
-            for (int sl = 0; sl < p.S; ++sl) {
-                if (!(present >> sl & 1)) continue;
-                for (int kk = 0; kk < r16 / 16; ++kk) {
-                    const uint32_t at = (sl * chunks + (kk >> 2)) * LT_TILE;
-                    const uint64_t bdesc = smem_desc_sw128(bbuf + at) + 2 * (kk & 3);
-                    tc_mma(d2, smem_desc_sw128(base + at) + 2 * (kk & 3), bdesc, idesc, more);
-                    more = 1;
-                    tc_mma(d2, smem_desc_sw128(base + hbytes + at) + 2 * (kk & 3), bdesc, idesc, 1);
+            if (lane == 0) {
+                const uint32_t at = ring + s * out_stage_bytes + LT_Y_BYTES;
+                for (int sl = 0; sl < p.S; ++sl) {
+                    if (!(present >> sl & 1)) continue;
+                    const uint32_t d = tmem + (acc * p.S + sl) * LT_COLS, h = base + sl * chunks * LT_TILE;
+                    for (int kk = 0; kk < steps; ++kk) {
+                        const uint64_t bdesc = smem_desc_sw128(at + (kk >> 2) * LT_TILE) + 2 * (kk & 3);
+                        tc_mma(d, smem_desc_sw128(h + (kk >> 2) * LT_TILE) + 2 * (kk & 3), bdesc, idesc, kk != 0);
+                        tc_mma(d, smem_desc_sw128(h + hbytes + (kk >> 2) * LT_TILE) + 2 * (kk & 3), bdesc, idesc, 1);
+                    }
+                }
+                tc_commit(s_addr(&acc_full[acc]));
+            }
+            __syncwarp();
+        }
+    } else {
+        const float scale = p.scale[e];
+        int i = 0;
+        for (int t = rank; t < tiles; t += C, ++i) {
+            const int s = i % out_stages, acc = i % accs, n0 = t * LT_COLS;
+            // lane j < 8: the slice of this warp's group j of 8 columns
+            const int n = n0 + half * 64 + (lane & 7) * 8;
+            const int own = p.col_slice != nullptr && n < p.N ? min((int)__ldg(p.col_slice + n / 8), p.S - 1) : 0;
+            bool ok = mbar_wait(s_addr(&out_full[s]), (i / out_stages) & 1, &abort_flag, p.status, wait_ns);
+            ok = ok && mbar_wait(s_addr(&acc_full[acc]), (i / accs) & 1, &abort_flag, p.status, wait_ns);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            unsigned char* stage = smem + 2 * hbytes + s * out_stage_bytes;
+            if (ok) {
+                unsigned char* mine = stage + half * LT_TILE;
+                const int row = quarter * 32 + lane;
+                const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + acc * p.S * LT_COLS + half * 64;
+#pragma unroll
+                for (int g0 = 0; g0 < 8; g0 += 4) {
+                    uint32_t v[32];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        lt_ld8(from + __shfl_sync(0xffffffffu, own, g0 + g) * LT_COLS + (g0 + g) * 8, v + g * 8);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        uint4* q = reinterpret_cast<uint4*>(mine + lt_swizzled(row, g0 + g));
+                        const uint4 a = *q;
+                        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
+                        uint4 o;
+                        uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            w[j] = pack_bf16(fmaf(scale, __uint_as_float(v[g * 8 + 2 * j]), __low2float(h[j])),
+                                             fmaf(scale, __uint_as_float(v[g * 8 + 2 * j + 1]), __high2float(h[j])));
+                        *q = o;
+                    }
                 }
             }
-            tc_commit(done);
-        }
-        if (n1 < p.N) fetch_y(n1, buf ^ 1);
-        const unsigned next = n1 < p.N ? slices_of(n1) : 0u;
-        mbar_wait(done, phase & 1, &abort_flag, p.status, wait_ns);
-        ++phase;
-        tc_fence_after();
-        if (n1 < p.N) fetch_b(n1, next);
-        cp_async_commit();
-        {
-            unsigned char* yrow = ymem + buf * LT_Y_BYTES + (quarter * 32 + lane) * LT_Y_ROW + half * 128;
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_addr(&acc_empty[acc]));
+            asm volatile("bar.sync 1, %0;" ::"n"(LT_EPI * 32) : "memory");
+            // rows in whole lines: 16 lanes a row
+            const int chunk = et & 15, col = n0 + chunk * 8;
+            if (ok && col < p.N) {
+                const unsigned char* from = stage + (chunk >> 3) * LT_TILE;
 #pragma unroll
-            for (int c0 = 0; c0 < 64; c0 += 32) {
-                uint32_t v[32];
-                __syncwarp();
-                tc_ld32(d2 + ((uint32_t)(quarter * 32) << 16) + half * 64 + c0, v);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    uint4* q = reinterpret_cast<uint4*>(yrow + (c0 + i) * 2);
-                    const uint4 a = *q;
-                    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
-                    uint4 o;
-                    uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        w[j] = pack_bf16(fmaf(scale, __uint_as_float(v[i + 2 * j]), __low2float(h[j])),
-                                         fmaf(scale, __uint_as_float(v[i + 2 * j + 1]), __high2float(h[j])));
-                    *q = o;
-                }
-            }
-        }
-        tc_fence_before();
-        __syncthreads();
-        {
-            const int chunk = tid & 15, n = n0 + chunk * 8;
-            if (n < p.N)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = (tid >> 4) + 16 * i;
+                for (int j = 0; j < 8; ++j) {
+                    const int row = (et >> 4) + 16 * j;
                     if (tok[row] >= 0)
-                        *reinterpret_cast<uint4*>(out + (size_t)tok[row] * p.N + n) =
-                            *reinterpret_cast<const uint4*>(ymem + buf * LT_Y_BYTES + row * LT_Y_ROW + chunk * 16);
+                        *reinterpret_cast<uint4*>(out + (size_t)tok[row] * p.N + col) = *reinterpret_cast<const uint4*>(from + lt_swizzled(row, chunk & 7));
                 }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_addr(&out_empty[s]));
         }
-        present = next;
-        buf ^= 1;
     }
-    cp_async_wait<0>();
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(d1), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
+}
+
+// A map of a row-major matrix [rows, cols] in boxes of box_rows x 64 columns with the 128-byte swizzle; made anew for every call.
+static int lora_map(CUtensorMap* map, const void* ptr, long long rows, int cols, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return fail(-4, "lora_add: the driver does not export cuTensorMapEncodeTiled");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols * 2};
+    const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows}, step[2] = {1u, 1u};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(-4, "lora_add: cuTensorMapEncodeTiled failed with code %d for a %lld x %d matrix", (int)r, rows, cols);
+    return 0;
 }
 
 int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream) {
@@ -346,14 +406,24 @@ int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream) {
     int C = 8;
     while (C > 1 && (tiles * C > sms || (p.K + 63) / 64 < C)) C /= 2;
     FD_REQUIRE(tiles * C < (1ll << 31), -2, "lora_add: %d tokens", p.T);
+    FD_REQUIRE((long long)p.E * p.N < (1ll << 31) && (long long)p.E * p.S * p.R < (1ll << 31), -2, "lora_add: %d adapters of %d rows", p.E, p.N);
+    LoraMaps maps;
+    int rc = lora_map(&maps.a, p.a, (long long)p.E * p.S * p.R, p.K, (p.R + 15) / 16 * 16);
+    if (rc == 0) rc = lora_map(&maps.b, p.b, (long long)p.E * p.N, p.R, LT_COLS);
+    const int boxes[3] = {LT_ROWS, 16, 1};
+    for (int i = 0; i < 3 && rc == 0; ++i) {
+        rc = lora_map(&maps.x[i], p.x, p.T, p.K, boxes[i]);
+        if (rc == 0) rc = lora_map(&maps.y[i], p.y, p.T, p.N, boxes[i]);
+    }
+    if (rc != 0) return rc;
     static Once once;
     if (once.first()) {
         const cudaError_t err = cudaFuncSetAttribute(lora_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_SMEM);
         if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
         once.done();
     }
-    return launch("lora_add", lora_tile_kernel, dim3((unsigned)(tiles * C)), dim3(LT_THREADS), f.smem, stream, dim3(C, 1, 1), p, f.chunks, f.stages,
-                  g_tc_wait_ns);
+    return launch("lora_add", lora_tile_kernel, dim3((unsigned)(tiles * C)), dim3(LT_THREADS), f.smem, stream, dim3(C, 1, 1), maps, p, f.chunks,
+                  f.stages, f.out_stages, g_tc_wait_ns);
 }
 
 }  // namespace fd
