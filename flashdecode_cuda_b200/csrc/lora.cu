@@ -10,6 +10,8 @@
 
 #include "lora.cuh"
 
+extern "C" int fd_sm_count();
+
 namespace fd {
 
 namespace cg = cooperative_groups;
@@ -37,7 +39,7 @@ template <typename T> __device__ __forceinline__ void load4(const T* p, float v[
 
 template <typename T>
 __global__ void __launch_bounds__(LR_THREADS)
-lora_general_kernel(const LoraArgs p) {
+lora_general_kernel(const LoraArgs p, int copies) {
     extern __shared__ __align__(16) float lr_smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -48,7 +50,7 @@ lora_general_kernel(const LoraArgs p) {
     __shared__ int tok[LR_ROWS];
     __shared__ LoraTile tile_s;
     if (warp == 0) {
-        const LoraTile f = lora_tile(p, blockIdx.x / C, LR_ROWS);
+        const LoraTile f = lora_tile(p, blockIdx.x / (C * copies), LR_ROWS);
         if (lane < LR_ROWS) {
             int t = lane < f.count ? p.order[f.begin + lane] : -1;
             if (lane < f.count && (t < 0 || t >= p.T)) { set_status(p.status, STATUS_BAD_INDEX); t = -1; }
@@ -60,7 +62,7 @@ lora_general_kernel(const LoraArgs p) {
     const LoraTile tile = tile_s;
     if (tile.adapter == -2) return;                              // the same for the whole cluster
     // this CTA's columns of the output
-    const int per = (((p.N + 7) / 8 + C - 1) / C) * 8, n0 = rank * per, n1 = min(p.N, n0 + per);
+    const int shares = C * copies, per = (((p.N + 7) / 8 + shares - 1) / shares) * 8, n0 = min(p.N, (int)(blockIdx.x % shares) * per), n1 = min(p.N, n0 + per);
     const T* y = static_cast<const T*>(p.y);
     T* out = static_cast<T*>(p.out);
     if (tile.adapter < 0) {
@@ -184,24 +186,31 @@ static int launch_general(const LoraArgs& p, cudaStream_t stream) {
     const int C = lora_cluster(p), W = p.S * ((p.R + 3) & ~3);
     const size_t smem = sizeof(float) * (LR_ROWS * LR_CHUNK + 2 * (size_t)LR_ROWS * W);
     const long long tiles = lora_max_tiles(p, LR_ROWS);
-    FD_REQUIRE(tiles * C < (1ll << 31), -2, "lora_add: %d tokens", p.T);
+    // where the tiles leave SMs idle, several clusters share a tile's columns (each computes the same A x)
+    int copies = (int)(2 * fd_sm_count() / (tiles * C));
+    while (copies > 1 && p.N < LR_THREADS * C * copies) --copies;
+    if (copies < 1) copies = 1;
+    FD_REQUIRE(tiles * C * copies < (1ll << 31), -2, "lora_add: %d tokens", p.T);
     static Once once;
     if (once.first()) {
         const cudaError_t err = cudaFuncSetAttribute(lora_general_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
         if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
         once.done();
     }
-    return launch("lora_add", lora_general_kernel<T>, dim3((unsigned)(tiles * C)), dim3(LR_THREADS), smem, stream, dim3(C, 1, 1), p);
+    return launch("lora_add", lora_general_kernel<T>, dim3((unsigned)(tiles * C * copies)), dim3(LR_THREADS), smem, stream, dim3(C, 1, 1), p, copies);
 }
 
 }  // namespace fd
 
 using namespace fd;
 
-extern "C" int fd_sm_count();
-
-// Tokens per segment, on average, from which tiles of 128 are taken.
-constexpr int LORA_TILE_TOKENS = 32;
+// Tiles of 128 are taken for so many tokens of a step, and of a segment on average (the adapters' tokens are known on the device only),
+// where tiles of 16 would read so many bytes of A and B (out of L2, most of them).  Measured, tiles of 16 / of 128, us: q/k/v of
+// 1536 x 2048, rank 16, 2,048 tokens (27 MB) 19 / 22, 4,096 (55 MB) 30 / 24; 3584 x 3584, rank 32, 2,048 (59 MB) 26 / 30, 4,096 41 / 31;
+// 13824 x 5120, rank 64, 512 (78 MB) 24 / 34, 1,024 35 / 34, 4,096 110 / 56; 3584 x 37888 in two slices, rank 64, 512 (185 MB) 61 / 94,
+// 1,024 102 / 95, 4,096 377 / 169.
+constexpr int LORA_TILE_TOKENS = 1024, LORA_TILE_SEGMENT = 64;
+constexpr long long LORA_TILE_BYTES = 64000000;
 
 static int g_lora_form = 0;
 // Which form the bfloat16 steps on the tensor cores take from now on: 1 = tiles of 16 tokens, 2 = tiles of 128 where they take the
@@ -223,7 +232,8 @@ extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const fl
     const LoraArgs p{x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status, T, K, N, E, R, S, n_seg};
     if (dtype == 0) return launch_general<float>(p, stream);
     if (!lora_mma_takes(p)) return launch_general<__nv_bfloat16>(p, stream);
-    // (the adapters' tokens are known on the device only: by their average)
-    const bool many = g_lora_form == 0 ? T >= LORA_TILE_TOKENS * n_seg : g_lora_form == 2;
+    const bool many = g_lora_form == 0 ? T >= LORA_TILE_TOKENS && T / n_seg >= LORA_TILE_SEGMENT &&
+                                             (long long)(T / 16) * 2 * R * ((long long)S * K + N) >= LORA_TILE_BYTES
+                                       : g_lora_form == 2;
     return many && lora_tiles_take(p) ? lora_tiles(p, fd_sm_count(), stream) : lora_rows(p, fd_sm_count(), stream);
 }

@@ -81,10 +81,10 @@ __device__ __forceinline__ uint4 lora_sum8(const uint4& y, const float v[8], flo
 // columns of its token: y and out move 16 bytes at a time, and a pass of 32 columns is two loads and two stores per lane beside the
 // weights.  The groups are neighbours, or every other one where two slices take turns (gate and up).
 // What bounds it is the load and store pipe (a warp's 16 bytes per lane are eight rows' 64 bytes) beside the memory, so h stays in
-// registers from pass to pass, and nothing is selected where what is read does no harm: rows of no token read token 0's y and are not
+// registers from pass to pass (for ranks up to 64), and nothing is selected where what is read does no harm: rows of no token read token 0's y and are not
 // stored, groups behind n1 read the last one's weights, chunks behind the rank the first one's against zeros in h.
-// NC: chunks of 32 places that h may have (the rank is at most 32 NC).
-template <int NC, bool TWO>
+// NC: chunks of 32 places of h at once; HELD: those are all there are (the rank is at most 32 NC), and stay.
+template <int NC, bool TWO, bool HELD = true>
 __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat16* b, const __nv_bfloat16* y, __nv_bfloat16* out,
                                             const __nv_bfloat16* hi, const __nv_bfloat16* lo, int WB, int t0, int t1, int n0, int n1,
                                             int r8, float scale) {
@@ -97,6 +97,7 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat
     const __nv_bfloat16* bp = b + (size_t)(g & 1) * p.R + q * 8;
     int held = -1;                                               // the slice that f is of
     LoraFrag<TWO> f[NC];
+    int border = 0;
     // passes come in pairs that share 64 columns
     for (int pass = warp; ; pass += LM_WARPS) {
         const int base = n0 + (pass >> 1) * 64, half = pass & 1;
@@ -119,54 +120,42 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat
         }
         if (first >= n1) continue;
         const int og = first + q * step, wg = min(first + (g >> 1) * step, n1 - 8);            // the lane's group of outputs, and of weights
-        const bool in = og < n1;
-        if (!one) {
-            // a border between slices inside the four groups: each lane's group by itself, in plain arithmetic
-            if (in) {
-                const __nv_bfloat16* hs = hi + min((int)__ldg(p.col_slice + og / 8), p.S - 1) * Rc;
-                for (int k = 0; k < (TWO ? 2 : 1); ++k) {
-                    const int t = k ? t1 : t0;
-                    if (t < 0) continue;
-                    const __nv_bfloat16* ht = hs + (g + 8 * k) * WB;
-                    for (int n = og; n < og + 8; ++n) {
-                        float v = 0.f;
-                        for (int j = 0; j < r8; ++j) v = fmaf(__bfloat162float(ht[j]) + __bfloat162float(ht[j + low]), __bfloat162float(b[(size_t)n * p.R + j]), v);
-                        const size_t o = (size_t)t * p.N + n;
-                        out[o] = __float2bfloat16_rn(fmaf(scale, v, __bfloat162float(y[o])));
-                    }
-                }
-            }
-            continue;
+        bool in = og < n1;
+        if (!one) {                                              // a border between slices inside the four groups: a pass for each slice,
+            slice = border;                                      // which stores the groups that are its own
+            in = in && min((int)__ldg(p.col_slice + og / 8), p.S - 1) == slice;
         }
         const __nv_bfloat16* wp = bp + (size_t)wg * p.R;
-        uint4 w[NC][4];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            if (NC > 1 && c * 32 >= r8) break;
-            const int j = c * 32 + q * 8 < r8 ? c * 32 : -q * 8;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[c][i] = ldg16(wp + 2 * i * p.R + j);
-        }
         uint4 y0 = make_uint4(0u, 0u, 0u, 0u), y1 = y0;
-        if (in) {
-            y0 = *reinterpret_cast<const uint4*>(yp0 + og);
-            if (TWO) y1 = *reinterpret_cast<const uint4*>(yp1 + og);
-        }
-        if (slice != held) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) f[c].load(h + slice * Rc + min(c * 32, Rc - 32), low, up);
-            held = slice;
-        }
         float acc[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+        for (int j0 = 0; j0 < (HELD ? 1 : r8); j0 += 32 * NC) {
+            uint4 w[NC][4];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            if (NC > 1 && c * 32 >= r8) break;
+            for (int c = 0; c < NC; ++c) {
+                if (NC > 1 && j0 + c * 32 >= r8) break;
+                const int j = j0 + c * 32 + q * 8 < r8 ? j0 + c * 32 : -q * 8;
 #pragma unroll
-            for (int m = 0; m < LoraFrag<TWO>::STEPS; ++m)
+                for (int i = 0; i < 4; ++i) w[c][i] = ldg16(wp + 2 * i * p.R + j);
+            }
+            if (in && j0 == 0) {
+                y0 = *reinterpret_cast<const uint4*>(yp0 + og);
+                if (TWO) y1 = *reinterpret_cast<const uint4*>(yp1 + og);
+            }
+            if (!HELD || slice != held) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[c].mma(m, acc[i], w[c][i]);
+                for (int c = 0; c < NC; ++c) f[c].load(h + slice * Rc + min(j0 + c * 32, Rc - 32), low, up);
+                held = slice;
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if (NC > 1 && j0 + c * 32 >= r8) break;
+#pragma unroll
+                for (int m = 0; m < LoraFrag<TWO>::STEPS; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[c].mma(m, acc[i], w[c][i]);
+            }
         }
         if (in) {
             float v[8];
@@ -183,6 +172,8 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat
                 if (t1 >= 0) *reinterpret_cast<uint4*>(op1 + og) = lora_sum8(y1, v, scale);
             }
         }
+        if (!one && ++border < p.S) pass -= LM_WARPS;
+        else border = 0;
     }
 }
 
@@ -323,11 +314,11 @@ lora_rows_kernel(const LoraArgs p, int copies) {
     if (tile.count > 8) {
         if (r8 <= 32) lora_expand<1, true>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
         else if (r8 <= 64) lora_expand<2, true>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
-        else lora_expand<4, true>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
+        else lora_expand<2, true, false>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
     } else {
         if (r8 <= 32) lora_expand<1, false>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
         else if (r8 <= 64) lora_expand<2, false>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
-        else lora_expand<4, false>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
+        else lora_expand<2, false, false>(p, b, y, out, hi, lo, WB, t0, t1, n0, n1, r8, scale);
     }
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");          // this CTA's sums have been read by all

@@ -403,7 +403,8 @@ static int lora_map(CUtensorMap* map, const void* ptr, long long rows, int cols,
 int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream) {
     const LoraTilePlan f = lora_tile_plan(p);
     const long long tiles = lora_max_tiles(p, LT_ROWS);
-    int C = 8;
+    // (clusters of 8 with an SM for each CTA find room two to a group of 16 to 18 SMs: 17 of them take two waves)
+    int C = tiles <= 16 ? 8 : 4;
     while (C > 1 && (tiles * C > sms || (p.K + 63) / 64 < C)) C /= 2;
     FD_REQUIRE(tiles * C < (1ll << 31), -2, "lora_add: %d tokens", p.T);
     FD_REQUIRE((long long)p.E * p.N < (1ll << 31) && (long long)p.E * p.S * p.R < (1ll << 31), -2, "lora_add: %d adapters of %d rows", p.E, p.N);
