@@ -18,7 +18,7 @@ namespace cg = cooperative_groups;
 
 constexpr int LR_THREADS = 256, LR_WARPS = LR_THREADS / 32;
 constexpr int LR_ROWS = 16;              // tokens of a tile
-constexpr int LR_CHUNK = 512;            // columns of x in shared memory at once
+constexpr int LR_CHUNK = 1024;           // columns of x in shared memory at once
 constexpr int LR_J = 4;                  // rows of A that a warp multiplies at once: each x out of shared memory is used four times
 
 template <typename T> __device__ __forceinline__ void load4(const T* p, float v[4], bool whole, int n) {
@@ -37,16 +37,22 @@ template <typename T> __device__ __forceinline__ void load4(const T* p, float v[
     for (int e = 0; e < 4; ++e) v[e] = e < n ? to_float(p[e]) : 0.f;
 }
 
+// Floats per token for a CTA's sums: every row of A, or the few of a small rank once for each of the warps that share them.
+__host__ __device__ __forceinline__ int lora_sums(int S, int R) {
+    const int all = (S * R + LR_J - 1) / LR_J * LR_J;
+    return all < LR_J * LR_WARPS ? LR_J * LR_WARPS : all;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(LR_THREADS)
-lora_general_kernel(const LoraArgs p, int copies) {
+lora_general_kernel(const LoraArgs p, int copies, int chunk) {
     extern __shared__ __align__(16) float lr_smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int Rp = (p.R + 3) & ~3, W = p.S * Rp;                 // a token's A x: S slices of Rp places
-    float* xs = lr_smem;                                         // [LR_ROWS][LR_CHUNK]
-    float* part = xs + LR_ROWS * LR_CHUNK;                       // [LR_ROWS][W] this CTA's sums
-    float* h = part + LR_ROWS * W;                               // [LR_ROWS][W] the cluster's
+    float* xs = lr_smem;                                         // [LR_ROWS][chunk]
+    float* part = xs + LR_ROWS * chunk;                       // [parts][LR_ROWS][U] this CTA's sums, of the rows of A that the adapter has
+    float* h = part + LR_ROWS * lora_sums(p.S, p.R);             // [LR_ROWS][W] the cluster's
     __shared__ int tok[LR_ROWS];
     __shared__ LoraTile tile_s;
     if (warp == 0) {
@@ -76,41 +82,43 @@ lora_general_kernel(const LoraArgs p, int copies) {
     if (r == 0 && static_cast<const void*>(out) == p.y) return;   // an adapter that leaves this projection alone
     const T* x = static_cast<const T*>(p.x);
     const T* a = static_cast<const T*>(p.a) + (size_t)e * p.S * p.R * p.K;
-    for (int i = tid; i < LR_ROWS * W; i += LR_THREADS) part[i] = 0.f;
+    // Groups of LR_J rows of A for the warps; those that are left over share a group's columns.  (By the adapter's rank and the sizes.)
+    const int kper = (((p.K + 3) / 4 + C - 1) / C) * 4, k0 = rank * kper, k1 = min(p.K, k0 + kper);
+    const int U = (p.S * r + LR_J - 1) / LR_J * LR_J, groups = U / LR_J;
+    const int parts = max(1, min(LR_WARPS / max(groups, 1), (kper + 127) / 128));
+    for (int i = tid; i < parts * LR_ROWS * U; i += LR_THREADS) part[i] = 0.f;
 
     // --- A x over this CTA's share of K
-    const int kper = (((p.K + 3) / 4 + C - 1) / C) * 4, k0 = rank * kper, k1 = min(p.K, k0 + kper);
     constexpr unsigned long long unit = 4 * sizeof(T) - 1;       // rows that begin where four values can be loaded at once
     const bool whole4 = (p.K & 3) == 0 && ((reinterpret_cast<unsigned long long>(p.x) | reinterpret_cast<unsigned long long>(p.a)) & unit) == 0;
-    for (int c0 = k0; c0 < k1; c0 += LR_CHUNK) {
-        const int w = min(LR_CHUNK, k1 - c0), w4 = (w + 3) / 4;
+    for (int c0 = k0; c0 < k1; c0 += chunk) {
+        const int w = min(chunk, k1 - c0), w4 = (w + 3) / 4;
         __syncthreads();
         for (int i = tid; i < LR_ROWS * w4; i += LR_THREADS) {
             const int row = i / w4, c = (i - row * w4) * 4;
             float v[4] = {0.f, 0.f, 0.f, 0.f};
             if (tok[row] >= 0) load4(x + (size_t)tok[row] * p.K + c0 + c, v, whole4, w - c);
-            *reinterpret_cast<float4*>(xs + row * LR_CHUNK + c) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(xs + row * chunk + c) = make_float4(v[0], v[1], v[2], v[3]);
         }
         __syncthreads();
-        for (int u0 = warp * LR_J; u0 < p.S * r; u0 += LR_WARPS * LR_J) {
+        for (int gi = warp; gi < groups * parts; gi += LR_WARPS) {
+            const int u0 = gi / parts * LR_J, mine = gi % parts;
             float acc[LR_J * LR_ROWS];
 #pragma unroll
             for (int i = 0; i < LR_J * LR_ROWS; ++i) acc[i] = 0.f;
             const T* rows[LR_J];
-            int place[LR_J];
 #pragma unroll
             for (int j = 0; j < LR_J; ++j) {
                 const int u = min(u0 + j, p.S * r - 1), s = u / r;
                 rows[j] = a + (size_t)(s * p.R + (u - s * r)) * p.K + c0;
-                place[j] = u0 + j < p.S * r ? s * Rp + (u - s * r) : -1;
             }
-            for (int c = lane * 4; c < w; c += 128) {
+            for (int c = mine * 128 + lane * 4; c < w; c += parts * 128) {
                 float av[LR_J][4];
 #pragma unroll
                 for (int j = 0; j < LR_J; ++j) load4(rows[j] + c, av[j], whole4, w - c);
 #pragma unroll
                 for (int i = 0; i < LR_ROWS; ++i) {
-                    const float4 xv = *reinterpret_cast<const float4*>(xs + i * LR_CHUNK + c);
+                    const float4 xv = *reinterpret_cast<const float4*>(xs + i * chunk + c);
 #pragma unroll
                     for (int j = 0; j < LR_J; ++j)
                         acc[j * LR_ROWS + i] += av[j][0] * xv.x + av[j][1] * xv.y + av[j][2] * xv.z + av[j][3] * xv.w;
@@ -131,17 +139,32 @@ lora_general_kernel(const LoraArgs p, int copies) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int j = (first + i) / LR_ROWS, row = (first + i) % LR_ROWS;
-                int pl = place[0];
-#pragma unroll
-                for (int q = 1; q < LR_J; ++q) pl = j == q ? place[q] : pl;
-                if (pl >= 0) part[row * W + pl] += acc[i];
+                part[(mine * LR_ROWS + row) * U + u0 + j] += acc[i];               // (rows behind the rank: the last one's once more)
             }
+        }
+    }
+    if (parts > 1) {
+        __syncthreads();
+        for (int i = tid; i < LR_ROWS * U; i += LR_THREADS) {
+            float v = part[i];
+            for (int q = 1; q < parts; ++q) v += part[q * LR_ROWS * U + i];
+            part[i] = v;
         }
     }
     cluster.sync();
     for (int i = tid; i < LR_ROWS * W; i += LR_THREADS) {
+        const int row = i / W, pl = i - row * W, s = pl / Rp, j = pl - s * Rp;
         float v = 0.f;
-        for (int c = 0; c < C; ++c) v += *cluster.map_shared_rank(part + i, c);
+        if (j < r && row < tile.count) {
+            const float* f = part + row * U + s * r + j;
+            if (C == 16) {                                       // all in flight at once
+#pragma unroll
+                for (int c = 0; c < 16; ++c) v += *cluster.map_shared_rank(f, c);
+            } else {
+#pragma unroll 4
+                for (int c = 0; c < C; ++c) v += *cluster.map_shared_rank(f, c);
+            }
+        }
         h[i] = v;
     }
     cluster.sync();                                              // the others' sums have been read, and h is whole
@@ -154,9 +177,13 @@ lora_general_kernel(const LoraArgs p, int copies) {
         const int s = p.col_slice != nullptr ? min((int)p.col_slice[n >> 3], p.S - 1) : 0;
         const T* bn = b + (size_t)n * p.R;
         const float* hs = h + s * Rp;
-        float acc[LR_ROWS];
+        // (all of y before the first store: out may be y, and each load would wait for the store before it)
+        float acc[LR_ROWS], yv[LR_ROWS];
 #pragma unroll
-        for (int i = 0; i < LR_ROWS; ++i) acc[i] = 0.f;
+        for (int i = 0; i < LR_ROWS; ++i) {
+            acc[i] = 0.f;
+            yv[i] = tok[i] >= 0 ? to_float(y[(size_t)tok[i] * p.N + n]) : 0.f;
+        }
         for (int j = 0; j < r; j += 4) {
             float bv[4];
             load4(bn + j, bv, vec, r - j);
@@ -168,23 +195,21 @@ lora_general_kernel(const LoraArgs p, int copies) {
         }
 #pragma unroll
         for (int i = 0; i < LR_ROWS; ++i)
-            if (i < tile.count && tok[i] >= 0) {
-                const size_t o = (size_t)tok[i] * p.N + n;
-                out[o] = from_float<T>(to_float(y[o]) + scale * acc[i]);
-            }
+            if (tok[i] >= 0) out[(size_t)tok[i] * p.N + n] = from_float<T>(yv[i] + scale * acc[i]);
     }
 }
 
 // CTAs of a cluster: enough to spread one tile's matrices, by the sizes alone.
 static int lora_cluster(const LoraArgs& p) {
     const int most = p.K > p.N ? p.K : p.N;
-    return most >= 1024 ? 8 : (most >= 512 ? 4 : (most >= 256 ? 2 : 1));
+    return p.K >= 4096 ? 16 : (most >= 1024 ? 8 : (most >= 512 ? 4 : (most >= 256 ? 2 : 1)));
 }
 
 template <typename T>
 static int launch_general(const LoraArgs& p, cudaStream_t stream) {
     const int C = lora_cluster(p), W = p.S * ((p.R + 3) & ~3);
-    const size_t smem = sizeof(float) * (LR_ROWS * LR_CHUNK + 2 * (size_t)LR_ROWS * W);
+    const int kper = (((p.K + 3) / 4 + C - 1) / C) * 4, chunk = kper < LR_CHUNK ? kper : LR_CHUNK;
+    const size_t smem = sizeof(float) * LR_ROWS * (chunk + (size_t)W + lora_sums(p.S, p.R));
     const long long tiles = lora_max_tiles(p, LR_ROWS);
     // where the tiles leave SMs idle, several clusters share a tile's columns (each computes the same A x)
     int copies = (int)(2 * fd_sm_count() / (tiles * C));
@@ -193,11 +218,12 @@ static int launch_general(const LoraArgs& p, cudaStream_t stream) {
     FD_REQUIRE(tiles * C * copies < (1ll << 31), -2, "lora_add: %d tokens", p.T);
     static Once once;
     if (once.first()) {
-        const cudaError_t err = cudaFuncSetAttribute(lora_general_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        cudaError_t err = cudaFuncSetAttribute(lora_general_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (err == cudaSuccess) err = cudaFuncSetAttribute(lora_general_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (err != cudaSuccess) return fail(-100, "lora_add: %s", cudaGetErrorString(err));
         once.done();
     }
-    return launch("lora_add", lora_general_kernel<T>, dim3((unsigned)(tiles * C * copies)), dim3(LR_THREADS), smem, stream, dim3(C, 1, 1), p, copies);
+    return launch("lora_add", lora_general_kernel<T>, dim3((unsigned)(tiles * C * copies)), dim3(LR_THREADS), smem, stream, dim3(C, 1, 1), p, copies, chunk);
 }
 
 }  // namespace fd

@@ -98,15 +98,24 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat
     int held = -1;                                               // the slice that f is of
     LoraFrag<TWO> f[NC];
     int border = 0;
-    // passes come in pairs that share 64 columns
+    // Passes come in pairs that share 64 columns.  Lane i knows the slice of group i of those (-1: behind the last): asked for a pass
+    // ahead, or each pass would be two trips to memory, one after the other.
+    auto slice_of = [&](int pass) {
+        const int n = n0 + (pass >> 1) * 64 + lane * 8;
+        return p.col_slice != nullptr && lane < 8 && n < n1 ? (int)__ldg(p.col_slice + n / 8) : -1;
+    };
+    int ahead = slice_of(warp), mine = ahead;
     for (int pass = warp; ; pass += LM_WARPS) {
         const int base = n0 + (pass >> 1) * 64, half = pass & 1;
         if (base >= n1) break;
+        if (border == 0) {
+            mine = ahead;
+            ahead = slice_of(pass + LM_WARPS);
+        }
         int step = 8, first = base + half * 32, slice = 0;
         bool one = true;                                         // all four groups are of one slice
         if (p.col_slice != nullptr) {
-            // lane i looks at group i of the eight
-            const int c = lane < 8 && base + lane * 8 < n1 ? min((int)__ldg(p.col_slice + base / 8 + lane), p.S - 1) : -1;
+            const int c = min(mine, p.S - 1);
             const int c0 = __shfl_sync(0xffffffffu, c, 0), c1 = __shfl_sync(0xffffffffu, c, 1), c4 = __shfl_sync(0xffffffffu, c, 4);
             const bool turns = __all_sync(0xffffffffu, c < 0 || c == (lane & 1 ? c1 : c0)) && c1 >= 0 && c0 != c1;
             if (turns) {
@@ -334,7 +343,7 @@ bool lora_mma_takes(const LoraArgs& p) {
 int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream) {
     const long long tiles = lora_max_tiles(p, LM_ROWS);
     const int most = p.K > p.N ? p.K : p.N;
-    int C = tiles * 16 <= sms ? 16 : 8;
+    int C = tiles * 16 <= LM_CTAS * sms ? 16 : 8;
     while (C > 1 && (tiles * C > LM_CTAS * sms || most < 64 * C)) C /= 2;
     // where that leaves SMs idle, several clusters share a tile's columns (and each computes A x: the second reads A from L2)
     int copies = (int)(LM_CTAS * sms / (tiles * C));
