@@ -332,19 +332,28 @@ __device__ void beam_pick(BeamShared& sh, const float* __restrict__ x, int V, in
         return beam_key(sh.off[b], v);
     };
     if (t == 0) sh.n_list = sh.n_found = sh.n_kept = 0;
-    unsigned long long mine[1] = {0ull};
-#pragma unroll 4
+    // the thread's largest, and its second: with few groups per thread hardly one has two that reach T
+    unsigned long long mine[1] = {0ull}, second = 0ull;
+    int where = 0;
+#pragma unroll 8
     for (int i = t; i < N; i += THREADS) {
         const unsigned long long q = group_key(i);
-        mine[0] = q > mine[0] ? q : mine[0];
+        const bool more = q > mine[0];
+        second = more ? mine[0] : (q > second ? q : second);
+        where = more ? i : where;
+        mine[0] = more ? q : mine[0];
     }
     unsigned long long T = beam_threshold(mine, k);
-    if (mine[0] >= T)
+    auto list = [&](int i) {
+        const int p = atomicAdd(&sh.n_list, 1);
+        if (p < BM_LIST) sh.list[p] = i;
+    };
+    if (second >= T) {
         for (int i = t; i < N; i += THREADS)
-            if (group_key(i) >= T) {
-                const int p = atomicAdd(&sh.n_list, 1);
-                if (p < BM_LIST) sh.list[p] = i;
-            }
+            if (group_key(i) >= T) list(i);
+    } else if (mine[0] >= T) {
+        list(where);
+    }
     __syncthreads();
     int ng = sh.n_list;
     const bool listed = ng <= BM_LIST;
