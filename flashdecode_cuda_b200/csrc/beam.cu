@@ -167,6 +167,7 @@ template <bool VEC, bool SMALL>
 __global__ void __launch_bounds__(BM_SCAN_THREADS)
 beam_scan_kernel(const float* __restrict__ logits, int V, int units, int groups, int per, float* __restrict__ gmax, float* __restrict__ part_m,
                  double* __restrict__ part_s) {
+    pdl_launch_dependents();                                   // the pick is set up while the last rows are read
     const int row = blockIdx.y, split = blockIdx.x, warp = threadIdx.x >> 5;
     float m = -INFINITY;
     double s = 0.0;
@@ -481,6 +482,7 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int n, const float* __
                  const double* __restrict__ part_s, int k, const BeamOut out, int* status) {
     __shared__ BeamShared sh;
     const int r = blockIdx.x;
+    pdl_wait();
     int first;
     const int nb = beam_rows(start, r, n, first, status);
     beam_none(out, r, k);
@@ -606,9 +608,7 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     else beam_scan_kernel<false, false><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
     int rc = check_launch("beam_select");
     if (rc != 0) return rc;
-    if (small)
-        beam_pick_kernel<BM_SMALL_GROUP><<<R, BM_PICK_THREADS, 0, stream>>>(logits, V, n, scores, start, groups, p.splits, gmax, part_m, part_s, k, out, status);
-    else
-        beam_pick_kernel<BM_GROUP><<<R, BM_PICK_THREADS, 0, stream>>>(logits, V, n, scores, start, groups, p.splits, gmax, part_m, part_s, k, out, status);
-    return check_launch("beam_select_pick");
+    return launch_with(true, "beam_select_pick", small ? beam_pick_kernel<BM_SMALL_GROUP> : beam_pick_kernel<BM_GROUP>, dim3(R),
+                       dim3(BM_PICK_THREADS), 0, stream, dim3(1, 1, 1), logits, V, n, scores, start, groups, p.splits, (const float*)gmax,
+                       (const float*)part_m, (const double*)part_s, k, out, status);
 }
