@@ -38,6 +38,7 @@ constexpr int BM_PICK_THREADS = 1024;
 constexpr int BM_CLUSTER_THREADS = 512;
 constexpr int BM_MAX_ROWS = 64;          // beams of one request
 constexpr int BM_MAX_K = 128;            // candidates of one request
+constexpr int BM_MAX_VOCAB = 1 << 22;    // so that the numbers of a request's groups and entries stay exact in 32 bits
 constexpr int BM_LIST = 512;             // groups that may reach T before the exact cut is taken
 constexpr int BM_FOUND = 2048;           // entries that may
 constexpr int BM_KEPT = 256;             // entries that are ranked (more than that many get a nearer threshold first)
@@ -252,8 +253,8 @@ struct BeamOut {
     int* tok;
 };
 
-// Division of small numbers (quotient and divisor below 2^16) by a number that is not known to the compiler: exact, since the quotient's
-// error in 32 bits is far below the distance of (i + 1/2) / d from a whole number.
+// Division by a number that is not known to the compiler, for numbers below 2^22, divisors up to 2^15 and quotients up to 2^6: i + 1/2
+// is exact, the quotient is off by less than 2^6 2^-22, and (i + 1/2) / d is at least 2^-16 from a whole number.
 struct BeamDiv {
     float inv;
     int d;
@@ -574,7 +575,7 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     FD_REQUIRE(n > 0 && V > 0 && R > 0, -2, "beam_select: %d rows of %d logits for %d requests", n, V, R);
     FD_REQUIRE(n <= 65535, -2, "beam_select: %d rows in one call", n);
     FD_REQUIRE(k >= 1 && k <= BM_MAX_K, -2, "beam_select: %d candidates per request; 1 to %d are taken", k, BM_MAX_K);
-    FD_REQUIRE((long long)V * BM_MAX_ROWS < (1ll << 31), -2, "beam_select: a vocabulary of %d", V);
+    FD_REQUIRE(V <= BM_MAX_VOCAB, -2, "beam_select: a vocabulary of %d; up to %d are taken", V, BM_MAX_VOCAB);
     const BeamOut out{out_s, out_row, out_tok};
     const bool small = V <= BM_SMALL_VOCAB;
     const bool vec = !small && V % 4 == 0 && (reinterpret_cast<unsigned long long>(logits) & 15) == 0;

@@ -53,6 +53,7 @@ class _Graph:
         self.logits: Optional[torch.Tensor] = None   # [bucket, vocab] float32: the step's logits, in the graph's workspace
         self.host: Optional[np.ndarray] = None       # the step's index array; only a few slices change per step
         self.meta: Optional[torch.Tensor] = None     # its device copy (fixed address)
+        self.used: Optional[List[int]] = None        # the adapters that the index array was last filled for, row by row
 
 
 class GraphDecoder:
@@ -109,8 +110,11 @@ class GraphDecoder:
         ahead, self._ahead = self._ahead, None
         if ahead is None or ahead[0] is not g or ahead[1] != tuple(slots) or ahead[2] != self.cache.lengths_version:
             self._fill_lengths(g, B, slots)     # else: written while the GPU ran the step before, and still true
-        if g.ctx.lora is not None:              # behind the wanted rows (all B of them)
-            h[8 * B:] = self.model.token_adapters(self.cache, slots, [1] * n, B, g.ctx.lora.ids.numel())
+        if g.ctx.lora is not None:              # behind the wanted rows (all B of them); the same for the same sequences' adapters
+            used = [self.cache.adapter(s) for s in slots]
+            if used != g.used:
+                h[8 * B:] = self.model.token_adapters(self.cache, slots, [1] * n, B, g.ctx.lora.ids.numel())
+                g.used = used
         self.model._staging.upload(h, g.meta)
 
     def _fill_lengths(self, g: _Graph, B: int, slots: Sequence[int]) -> None:
@@ -132,7 +136,7 @@ class GraphDecoder:
             return g, g.ctx
         if g is not None:
             ctx = self._prepare(g, key, slots, tokens)      # same bucket, another number of real rows
-            g.host, g.n_rows_real = self.model.last_meta_host.copy(), len(slots)
+            g.host, g.n_rows_real, g.used = self.model.last_meta_host.copy(), len(slots), None
             return g, ctx
         B = key[0]
         dev = self.model.device

@@ -1624,7 +1624,7 @@ def sample(logits: torch.Tensor, out: torch.Tensor, temperature: Optional[torch.
 # ---------------------------------------------------------------------------
 # requests of one batch that differ: several beams each, adapters of their own
 
-BEAM_MAX_ROWS, BEAM_MAX_CANDIDATES = 64, 128
+BEAM_MAX_ROWS, BEAM_MAX_CANDIDATES, BEAM_MAX_VOCAB = 64, 128, 1 << 22
 LORA_MAX_SLICES, LORA_MAX_RANK, LORA_MAX_PACKED = 4, 256, 512
 
 
@@ -1674,7 +1674,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, row_start: torch.Ten
     ``row_start[r + 1] - 1`` (int32 [R + 1]; at most BEAM_MAX_ROWS of them, none is allowed).  Its k best candidates
     scores[b] + log_softmax(logits[b])[v], best first, the lower row and then the lower token first where they tie, go to
     ``out_scores`` (float32), ``out_rows`` and ``out_tokens`` (int32), all [R, k] with k up to BEAM_MAX_CANDIDATES.  A logit of
-    -inf is no candidate; a row whose score or normaliser is no finite number (a NaN or +inf among its logits, nothing but -inf) has
+    -inf is no candidate; V is at most BEAM_MAX_VOCAB; a row whose score or normaliser is no finite number (a NaN or +inf among its logits, nothing but -inf) has
     none.  Places that no candidate fills: -inf, -1, -1.  ``scratch``: uint8 of ``beam_select_scratch_bytes(n, V)`` that the call may
     use; when omitted it is allocated."""
     f32, i32 = torch.float32, torch.int32
@@ -1772,5 +1772,7 @@ def lora_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Ten
         raise KernelError(f"lora_add: order, start and ids are int32 [{T}], [{n_seg + 1}], [{n_seg}]")
     if not (col_slice is None or (col_slice.dtype is torch.uint8 and col_slice.numel() * 8 == N)):
         raise KernelError("lora_add: col_slice is uint8 [N / 8]")
-    _check(lib().fd_lora_add(*_pointers(x, a, b, scale, ranks, order, start, ids, y, out, col_slice), _dt(dt), T, Kd, N, E, R, slices,
-                             n_seg, _ptr(status), _here_stream()))
+    at = _pointers(x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status)
+    if at[9] == at[0] and T:
+        raise KernelError("lora_add: out is x, which other tokens' products still read")
+    _check(lib().fd_lora_add(*at[:11], _dt(dt), T, Kd, N, E, R, slices, n_seg, at[11], _here_stream()))

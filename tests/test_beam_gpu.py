@@ -263,3 +263,34 @@ def test_both_forms(form, V, beams, k):
         check(x, torch.zeros(n), start, k)
     finally:
         K.beam_select_set_form(0)
+
+
+def test_two_kernels_in_a_graph_and_a_workspace_of_the_callers():
+    K.beam_select_set_form(2)
+    try:
+        g = torch.Generator().manual_seed(8)
+        a, b = (torch.randn(6, 50257, generator=g).to(DEV) for _ in range(2))
+        start, sc = torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV), torch.zeros(6, device=DEV)
+        want = [select(x.cpu(), torch.zeros(6), [0, 2, 6], 8) for x in (a, b)]
+        outs = [torch.empty(2, 8, device=DEV)] + [torch.empty(2, 8, dtype=torch.int32, device=DEV) for _ in range(2)]
+        scratch = torch.full((K.beam_select_scratch_bytes(6, 50257),), 255, dtype=torch.uint8, device=DEV)
+        x = a.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            K.beam_select(x, sc, start, *outs, scratch=scratch)
+        for src, w in ((b, want[1]), (a, want[0]), (b, want[1])):
+            x.copy_(src)
+            scratch.fill_(255)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p.cpu(), q) for p, q in zip(outs, w))
+    finally:
+        K.beam_select_set_form(0)
+
+
+def test_largest_vocabulary_and_beyond():
+    x = torch.zeros(2, K.BEAM_MAX_VOCAB)
+    x[0, -1], x[1, -129], x[1, 70000] = 3.0, 2.0, 2.0
+    check(x, torch.zeros(2), [0, 2], 4)
+    with pytest.raises(K.KernelError, match="vocabulary"):
+        select(torch.zeros(1, K.BEAM_MAX_VOCAB + 1), torch.zeros(1), [0, 1], 4)

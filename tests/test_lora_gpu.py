@@ -274,3 +274,59 @@ def test_both_forms(form, T, Kd, N, E, R, S, tiled):
         check("bfloat16", T, Kd, N, E, R, S, tiled, token=[(i // 150) % E for i in range(T)], in_place=True, seed=3)
     finally:
         K.lora_set_form(0)
+
+
+@pytest.mark.parametrize("form", [1, 2])
+@pytest.mark.parametrize("T", [300, 1500])
+def test_both_forms_on_other_streams_and_in_graphs(form, T):
+    K.lora_set_form(form)
+    try:
+        d, cols, S = make("bfloat16", T, 512, 776, 3, 32, 2, True)
+        tokens = [[(i // 70) % 4 - 1 for i in range(T)], [2 - (i // 200) % 3 for i in range(T)]]
+        wants = [run(d, cols, S, t) for t in tokens]
+        u = {k: v.to(DEV) for k, v in d.items()}
+        plans = [[p.clone() for p in plan(t)] for t in tokens]
+        # two graphs that share nothing, and whose replays overlap
+        graphs, outs, cs = [], [], cols.to(DEV)
+        for p in plans:
+            out, graph = torch.zeros_like(u["y"]), torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                K.lora_add(u["x"], u["a"], u["b"], u["scale"], u["ranks"], *p, u["y"], out, col_slice=cs, slices=S)
+            graphs.append(graph), outs.append(out)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        for _ in range(4):
+            for graph, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o.cpu(), w) for o, w in zip(outs, wants))
+    finally:
+        K.lora_set_form(0)
+
+
+def test_rows_that_lie_here_and_there():
+    """Prompts' tiles whose tokens are no neighbours: one by one, in runs of odd lengths, backwards."""
+    T = 1100
+    g = torch.Generator().manual_seed(11)
+    K.lora_set_form(2)
+    try:
+        for token in (torch.randint(0, 2, (T,), generator=g).tolist(), [(i // 37) % 2 for i in range(T)], [(i // 300) % 3 - 1 for i in range(T)]):
+            check("bfloat16", T, 456, 328, 2, 24, token=token)
+        d, cols, S = make("bfloat16", T, 456, 328, 2, 24)
+        u = {k: v.to(DEV) for k, v in d.items()}
+        up = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+        out = torch.zeros_like(u["y"])
+        K.lora_add(u["x"], u["a"], u["b"], u["scale"], u["ranks"], up(list(range(T - 1, -1, -1))), up([0, 500, T]), up([1, 0]), u["y"], out)
+        want, size, hsize = expected(d, cols, S, [0] * (T - 500) + [1] * 500)
+        assert bool(((out.cpu().double() - want).abs() <= tolerance("bfloat16", d, want, size, hsize)).all())
+    finally:
+        K.lora_set_form(0)
+
+
+def test_an_output_over_the_input_is_refused():
+    x = torch.zeros(3, 16, device=DEV)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)
+    with pytest.raises(K.KernelError, match="out is x"):
+        K.lora_add(x, torch.zeros(1, 4, 16, device=DEV), torch.zeros(1, 16, 4, device=DEV), torch.zeros(1, device=DEV), i(1), i(3), i(2), i(1),
+                   torch.zeros(3, 16, device=DEV), x)
