@@ -21,6 +21,7 @@ namespace cg = cooperative_groups;
 constexpr int LM_THREADS = 256, LM_WARPS = LM_THREADS / 32;
 constexpr int LM_ROWS = 16;              // tokens of a tile: the rows of an MMA
 constexpr int LM_CTAS = 2;               // per SM
+constexpr int LM_WIDE = 14;              // clusters of 16 that run at once
 constexpr int LM_TILES = 4;              // tiles of 8 rows of A that a warp accumulates at once
 constexpr int LM_RED = LM_TILES * 8 + 4; // floats of a token's row of a warp's sums (4: so that neighbouring rows are in other banks)
 
@@ -95,67 +96,85 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat
     const __nv_bfloat16 *yp0 = y + (size_t)max(t0, 0) * p.N, *yp1 = y + (size_t)max(t1, 0) * p.N;
     __nv_bfloat16 *op0 = out + (size_t)max(t0, 0) * p.N, *op1 = out + (size_t)max(t1, 0) * p.N;
     const __nv_bfloat16* bp = b + (size_t)(g & 1) * p.R + q * 8;
-    int held = -1;                                               // the slice that f is of
-    LoraFrag<TWO> f[NC];
-    int border = 0;
-    // Passes come in pairs that share 64 columns.  Lane i knows the slice of group i of those (-1: behind the last): asked for a pass
-    // ahead, or each pass would be two trips to memory, one after the other.
-    auto slice_of = [&](int pass) {
-        const int n = n0 + (pass >> 1) * 64 + lane * 8;
+    // Passes come in pairs that share 64 columns.  Lane i knows the slice of group i of those (-1: behind the last): asked for before
+    // the pass's weights, which are asked for before the pass before multiplies (where there are registers for both), or each
+    // pass would be two or three trips to memory, one after the other.
+    struct Pass {
+        int at, border, og, slice;
+        bool there, one, in;
+        uint4 w[NC][4], y0, y1;
+    };
+    constexpr bool EARLY = HELD && (NC == 1 || !TWO);
+    auto slice_of = [&](int at) {
+        const int n = n0 + (at >> 1) * 64 + lane * 8;
         return p.col_slice != nullptr && lane < 8 && n < n1 ? (int)__ldg(p.col_slice + n / 8) : -1;
     };
-    int ahead = slice_of(warp), mine = ahead;
-    for (int pass = warp; ; pass += LM_WARPS) {
-        const int base = n0 + (pass >> 1) * 64, half = pass & 1;
-        if (base >= n1) break;
-        if (border == 0) {
-            mine = ahead;
-            ahead = slice_of(pass + LM_WARPS);
+    auto weights = [&](Pass& s, int wg, int j0) {
+        const __nv_bfloat16* wp = bp + (size_t)wg * p.R;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (NC > 1 && j0 + c * 32 >= r8) break;
+            const int j = j0 + c * 32 + q * 8 < r8 ? j0 + c * 32 : -q * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s.w[c][i] = ldg16(wp + 2 * i * p.R + j);
         }
-        int step = 8, first = base + half * 32, slice = 0;
-        bool one = true;                                         // all four groups are of one slice
+    };
+    auto open = [&](Pass& s, int at, int border, int groups) -> int {
+        const int base = n0 + (at >> 1) * 64, half = at & 1;
+        s.at = at;
+        s.border = border;
+        s.there = base < n1;
+        if (!s.there) return 0;
+        int step = 8, first = base + half * 32;
+        s.slice = 0;
+        s.one = true;                                            // all four groups are of one slice
         if (p.col_slice != nullptr) {
-            const int c = min(mine, p.S - 1);
+            const int c = min(groups, p.S - 1);
             const int c0 = __shfl_sync(0xffffffffu, c, 0), c1 = __shfl_sync(0xffffffffu, c, 1), c4 = __shfl_sync(0xffffffffu, c, 4);
             const bool turns = __all_sync(0xffffffffu, c < 0 || c == (lane & 1 ? c1 : c0)) && c1 >= 0 && c0 != c1;
             if (turns) {
                 step = 16;
                 first = base + half * 8;
-                slice = half ? c1 : c0;
+                s.slice = half ? c1 : c0;
             } else {
-                slice = half ? c4 : c0;
-                one = __all_sync(0xffffffffu, c < 0 || (lane >> 2) != half || c == slice);
+                s.slice = half ? c4 : c0;
+                s.one = __all_sync(0xffffffffu, c < 0 || (lane >> 2) != half || c == s.slice);
             }
         }
-        if (first >= n1) continue;
-        const int og = first + q * step, wg = min(first + (g >> 1) * step, n1 - 8);            // the lane's group of outputs, and of weights
-        bool in = og < n1;
-        if (!one) {                                              // a border between slices inside the four groups: a pass for each slice,
-            slice = border;                                      // which stores the groups that are its own
-            in = in && min((int)__ldg(p.col_slice + og / 8), p.S - 1) == slice;
+        s.og = first + q * step;                                 // the lane's group of outputs
+        s.in = s.og < n1;
+        if (!s.one) {                                            // a border between slices inside the four groups: a pass for each slice,
+            s.slice = border;                                    // which stores the groups that are its own
+            s.in = s.in && min((int)__ldg(p.col_slice + s.og / 8), p.S - 1) == border;
         }
-        const __nv_bfloat16* wp = bp + (size_t)wg * p.R;
-        uint4 y0 = make_uint4(0u, 0u, 0u, 0u), y1 = y0;
+        s.slice = max(s.slice, 0);                               // (a pass behind n1 multiplies something, and stores nothing)
+        const int wg = min(first + (g >> 1) * step, n1 - 8);     // and of weights
+        weights(s, wg, 0);
+        if (s.in) {
+            s.y0 = *reinterpret_cast<const uint4*>(yp0 + s.og);
+            if (TWO) s.y1 = *reinterpret_cast<const uint4*>(yp1 + s.og);
+        }
+        return wg;
+    };
+    int held = -1;                                               // the slice that f is of
+    LoraFrag<TWO> f[NC];
+    Pass now, next;
+    int known = slice_of(warp), ahead = slice_of(warp + LM_WARPS);
+    int wg = open(now, warp, 0, known);
+    while (now.there) {
+        const bool again = !now.one && now.border + 1 < p.S;
+        const int at = again ? now.at : now.at + LM_WARPS, groups = again ? known : ahead;
+        int next_wg = 0;
+        if (EARLY) next_wg = open(next, at, again ? now.border + 1 : 0, groups);
         float acc[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
         for (int j0 = 0; j0 < (HELD ? 1 : r8); j0 += 32 * NC) {
-            uint4 w[NC][4];
+            if (j0 > 0) weights(now, wg, j0);
+            if (!HELD || now.slice != held) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                if (NC > 1 && j0 + c * 32 >= r8) break;
-                const int j = j0 + c * 32 + q * 8 < r8 ? j0 + c * 32 : -q * 8;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[c][i] = ldg16(wp + 2 * i * p.R + j);
-            }
-            if (in && j0 == 0) {
-                y0 = *reinterpret_cast<const uint4*>(yp0 + og);
-                if (TWO) y1 = *reinterpret_cast<const uint4*>(yp1 + og);
-            }
-            if (!HELD || slice != held) {
-#pragma unroll
-                for (int c = 0; c < NC; ++c) f[c].load(h + slice * Rc + min(j0 + c * 32, Rc - 32), low, up);
-                held = slice;
+                for (int c = 0; c < NC; ++c) f[c].load(h + now.slice * Rc + min(j0 + c * 32, Rc - 32), low, up);
+                held = now.slice;
             }
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -163,26 +182,34 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat
 #pragma unroll
                 for (int m = 0; m < LoraFrag<TWO>::STEPS; ++m)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) f[c].mma(m, acc[i], w[c][i]);
+                    for (int i = 0; i < 4; ++i) f[c].mma(m, acc[i], now.w[c][i]);
             }
         }
-        if (in) {
+        if (now.in) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) v[2 * i + e] = TWO ? acc[i][e] : acc[i][e] + acc[i][2 + e];
-            if (t0 >= 0) *reinterpret_cast<uint4*>(op0 + og) = lora_sum8(y0, v, scale);
+            if (t0 >= 0) *reinterpret_cast<uint4*>(op0 + now.og) = lora_sum8(now.y0, v, scale);
             if (TWO) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) v[2 * i + e] = acc[i][2 + e];
-                if (t1 >= 0) *reinterpret_cast<uint4*>(op1 + og) = lora_sum8(y1, v, scale);
+                if (t1 >= 0) *reinterpret_cast<uint4*>(op1 + now.og) = lora_sum8(now.y1, v, scale);
             }
         }
-        if (!one && ++border < p.S) pass -= LM_WARPS;
-        else border = 0;
+        if (EARLY) {
+            now = next;
+            wg = next_wg;
+        } else {
+            wg = open(now, at, again ? now.border + 1 : 0, groups);
+        }
+        if (!again) {
+            known = ahead;
+            ahead = slice_of(at + LM_WARPS);
+        }
     }
 }
 
@@ -343,7 +370,9 @@ bool lora_mma_takes(const LoraArgs& p) {
 int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream) {
     const long long tiles = lora_max_tiles(p, LM_ROWS);
     const int most = p.K > p.N ? p.K : p.N;
-    int C = tiles * 16 <= LM_CTAS * sms ? 16 : 8;
+    // Fourteen clusters of 16 run at once (groups of 16 or 18 SMs, two CTAs each); a fifteenth would double the time.  A segment's
+    // last tile is half full on average.
+    int C = p.n_seg <= LM_WIDE && p.T / LM_ROWS + (p.n_seg + 1) / 2 <= LM_WIDE ? 16 : 8;
     while (C > 1 && (tiles * C > LM_CTAS * sms || most < 64 * C)) C /= 2;
     // where that leaves SMs idle, several clusters share a tile's columns (and each computes A x: the second reads A from L2)
     int copies = (int)(LM_CTAS * sms / (tiles * C));

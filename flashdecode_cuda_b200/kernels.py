@@ -16,6 +16,7 @@ ordered with torch's own work and can be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
 from typing import Optional, Sequence
 
@@ -1727,12 +1728,15 @@ def copy_states(states: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Te
     m = len(at)
     if m == 0:
         return
-    slots = states[0].size(0) if states[0].dim() else -1
-    for t in states:
-        if not t.dim() or t.size(0) != slots:
-            raise KernelError("copy_states: the states are [slots, ...], all of one number of slots")
-    sizes = [t.nbytes for t in states]
-    _check(lib().fd_copy_states((c_void_p * m)(*at), (c_longlong * m)(*sizes), m, slots, s, d, n, st, _here_stream()))
+    try:
+        slots = states[0].size(0)
+        same = all([t.size(0) == slots for t in states])
+    except IndexError:
+        same = False
+    if not same:
+        raise KernelError("copy_states: the states are [slots, ...], all of one number of slots")
+    where, sizes = array("Q", at), array("q", [t.numel() * t.element_size() for t in states])
+    _check(lib().fd_copy_states(where.buffer_info()[0], sizes.buffer_info()[0], m, slots, s, d, n, st, _here_stream()))
 
 
 def lora_set_form(form: int) -> None:
