@@ -71,15 +71,16 @@ lora_general_kernel(const LoraArgs p, int copies, int chunk) {
     const int shares = C * copies, per = (((p.N + 7) / 8 + shares - 1) / shares) * 8, n0 = min(p.N, (int)(blockIdx.x % shares) * per), n1 = min(p.N, n0 + per);
     const T* y = static_cast<const T*>(p.y);
     T* out = static_cast<T*>(p.out);
-    if (tile.adapter < 0) {
+    const int e = max(tile.adapter, 0), r = tile.adapter < 0 ? 0 : min(max(p.ranks[e], 0), p.R);
+    if (r == 0) {                                                // nothing to add
         if (static_cast<const void*>(out) == p.y) return;
-        for (int i = 0; i < tile.count; ++i)
-            if (tok[i] >= 0)
-                for (int n = n0 + tid; n < n1; n += LR_THREADS) out[(size_t)tok[i] * p.N + n] = y[(size_t)tok[i] * p.N + n];
+        constexpr int per16 = 16 / (int)sizeof(T);               // n0 and n1 are multiples of 8, or N
+        if (p.N % per16 == 0 && ((reinterpret_cast<unsigned long long>(p.y) | reinterpret_cast<unsigned long long>(p.out)) & 15) == 0)
+            lora_copy<uint4>(tok, tile.count, p.y, p.out, p.N / per16, n0 / per16, n1 / per16, tid, LR_THREADS);
+        else
+            lora_copy<T>(tok, tile.count, p.y, p.out, p.N, n0, n1, tid, LR_THREADS);
         return;
     }
-    const int e = tile.adapter, r = min(max(p.ranks[e], 0), p.R);
-    if (r == 0 && static_cast<const void*>(out) == p.y) return;   // an adapter that leaves this projection alone
     const T* x = static_cast<const T*>(p.x);
     const T* a = static_cast<const T*>(p.a) + (size_t)e * p.S * p.R * p.K;
     // Groups of LR_J rows of A for the warps; those that are left over share a group's columns.  (By the adapter's rank and the sizes.)
@@ -252,6 +253,7 @@ extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const fl
     if (T == 0 || N == 0 || n_seg == 0) return 0;
     FD_REQUIRE(T > 0 && K > 0 && N > 0 && E > 0 && R > 0 && n_seg > 0, -2,
                "lora_add: %d tokens, %d x %d, %d adapters of rank %d, %d segments", T, K, N, E, R, n_seg);
+    FD_REQUIRE(K < (1 << 27) && N < (1 << 27), -2, "lora_add: %d x %d; up to 2^27 columns are taken", K, N);
     FD_REQUIRE(S >= 1 && S <= 4, -2, "lora_add: %d packed projections; 1 to 4 are taken", S);
     FD_REQUIRE(R <= 256 && S * R <= 512, -2, "lora_add: rank %d of %d packed projections; up to 256, and 512 in all, are taken", R, S);
     FD_REQUIRE(S == 1 || (col_slice != nullptr && N % 8 == 0), -2, "lora_add: %d packed projections need col_slice and N a multiple of 8", S);

@@ -69,6 +69,31 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& p, int tile, int r
     return f;
 }
 
+// Rows of tokens without an adapter (or of one that leaves the projection alone) as they are, for an output of its own: units u0 ..
+// u1 - 1 of `count` rows of `units`, by `threads` threads.  Eight loads of a thread before its first store: one after another, a
+// tile of 128 rows of 4,872 took 150 us, longer than any tile with products.
+template <typename U>
+__device__ __forceinline__ void lora_copy(const int* tok, int count, const void* from, void* to, int units, int u0, int u1, int t, int threads) {
+    const U* f = static_cast<const U*>(from);
+    U* o = static_cast<U*>(to);
+    const int width = u1 - u0, total = width > 0 ? width * count : 0;
+    for (int i0 = t; i0 < total; i0 += threads * 8) {
+        U v[8];
+        size_t at[8];
+        bool here[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * threads, row = i / width, token = i < total ? tok[row] : -1;
+            here[j] = token >= 0;
+            at[j] = here[j] ? (size_t)token * units + u0 + (i - row * width) : 0;
+            if (here[j]) v[j] = f[at[j]];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (here[j]) o[at[j]] = v[j];
+    }
+}
+
 // The most tiles there can be: every segment ends with one that may not be full.
 inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (long long)p.T / rows + p.n_seg; }
 

@@ -248,10 +248,7 @@ lora_rows_kernel(const LoraArgs p, int copies) {
     const int e = max(tile.adapter, 0), r = tile.adapter < 0 ? 0 : min(max(p.ranks[e], 0), p.R);
     if (r == 0) {                                                // nothing to add
         if (in_place) return;
-        for (int i = 0; i < tile.count; ++i)
-            if (tok[i] >= 0)
-                for (int n = n0 + tid * 8; n < n1; n += LM_THREADS * 8)
-                    *reinterpret_cast<uint4*>(out + (size_t)tok[i] * p.N + n) = *reinterpret_cast<const uint4*>(y + (size_t)tok[i] * p.N + n);
+        lora_copy<uint4>(tok, tile.count, p.y, p.out, p.N / 8, n0 / 8, n1 / 8, tid, LM_THREADS);
         return;
     }
     const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + (size_t)e * W * p.K;

@@ -152,12 +152,9 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
     const int e = max(tile.adapter, 0), r = tile.adapter < 0 ? 0 : min(max(p.ranks[e], 0), p.R);
     if (r == 0) {                                                // nothing to add
-        const __nv_bfloat16* y = static_cast<const __nv_bfloat16*>(p.y);
         if (static_cast<const void*>(out) == p.y) return;
-        for (int i = warp; i < tile.count; i += LT_THREADS / 32)
-            if (tok[i] >= 0)
-                for (int n = (rank * 32 + lane) * 8; n < p.N; n += C * 32 * 8)
-                    *reinterpret_cast<uint4*>(out + (size_t)tok[i] * p.N + n) = *reinterpret_cast<const uint4*>(y + (size_t)tok[i] * p.N + n);
+        const int per = (p.N / 8 + C - 1) / C, u0 = min(p.N / 8, rank * per);
+        lora_copy<uint4>(tok, tile.count, p.y, p.out, p.N / 8, u0, min(p.N / 8, u0 + per), tid, LT_THREADS);
         return;
     }
     if (warp == 1) {
