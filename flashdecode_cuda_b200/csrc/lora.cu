@@ -231,13 +231,25 @@ static int launch_general(const LoraArgs& p, cudaStream_t stream) {
 
 using namespace fd;
 
-// Tiles of 128 are taken for so many tokens of a step, and of a segment on average (the adapters' tokens are known on the device only),
-// where tiles of 16 would read so many bytes of A and B (out of L2, most of them).  Measured, tiles of 16 / of 128, us: q/k/v of
-// 1536 x 2048, rank 16, 2,048 tokens (27 MB) 19 / 22, 4,096 (55 MB) 30 / 24; 3584 x 3584, rank 32, 2,048 (59 MB) 26 / 30, 4,096 41 / 31;
-// 13824 x 5120, rank 64, 512 (78 MB) 24 / 34, 1,024 35 / 34, 4,096 110 / 56; 3584 x 37888 in two slices, rank 64, 512 (185 MB) 61 / 94,
-// 1,024 102 / 95, 4,096 377 / 169.
-constexpr int LORA_TILE_TOKENS = 1024, LORA_TILE_SEGMENT = 64;
-constexpr long long LORA_TILE_BYTES = 64000000;
+// Tiles of 128 are taken for segments of so many tokens on average (the adapters' tokens are known on the device only)
+//   * from LORA_TILE_TOKENS tokens on, where tiles of 16 would read LORA_TILE_BYTES of A and B (out of L2, most of them),
+//   * from LORA_TILE_FEW on, where they would read LORA_TILE_FEW_BYTES, if a tile gets a cluster of 8 or the slices' ranks add up to
+//     LORA_TILE_WIDE: between 16 and 20 tiles clusters of 4 leave half of the GPU idle, and tiles of 16 lose only if they multiply much.
+// Measured, tiles of 16 / of 128, us:
+//   3584 x 3584, rank 32: 1,024 tokens 13 / 19, 1,900 22 / 24, 2,048 22 / 29, 2,800 35 / 30, 4,096 36 / 31, 16,384 132 / 81
+//   2048 x 2560 in three slices, rank 16: 1,500 18 / 19, 2,048 20 / 23, 2,800 32 / 26, 16,384 121 / 62
+//   592 x 768 in two slices, rank 8: 2,800 12 / 15, 4,096 (8 MB) 12 / 16, 5,500 (11 MB) 19 / 18, 16,384 46 / 29
+//   4096 x 6144 in three slices, rank 16: 1,024 22 / 26, 1,500 (75 MB) 36 / 28, 2,048 37 / 39, 2,800 60 / 40
+//   3584 x 37888 in two slices, rank 16: 1,024 60 / 76, 1,500 106 / 77, 2,048 111 / 136; rank 64: 1,024 87 / 94, 1,500 155 / 96, 2,048 160 / 160
+//   13824 x 5120, rank 64: 512 23 / 32, 1,024 39 / 34, 2,048 66 / 52, 16,384 469 / 166
+constexpr int LORA_TILE_SEGMENT = 64, LORA_TILE_TOKENS = 2600, LORA_TILE_FEW = 1200, LORA_TILE_WIDE = 64;
+constexpr long long LORA_TILE_BYTES = 10000000, LORA_TILE_FEW_BYTES = 64000000;
+static bool lora_many(const LoraArgs& p) {
+    const long long bytes = (long long)(p.T / 16) * 2 * p.R * ((long long)p.S * p.K + p.N);
+    if (p.T / p.n_seg < LORA_TILE_SEGMENT) return false;
+    if (p.T >= LORA_TILE_TOKENS) return bytes >= LORA_TILE_BYTES;
+    return p.T >= LORA_TILE_FEW && bytes >= LORA_TILE_FEW_BYTES && (p.S * p.R >= LORA_TILE_WIDE || lora_tile_cluster(p, fd_sm_count()) == 8);
+}
 
 static int g_lora_form = 0;
 // Which form the bfloat16 steps on the tensor cores take from now on: 1 = tiles of 16 tokens, 2 = tiles of 128 where they take the
@@ -260,8 +272,6 @@ extern "C" int fd_lora_add(const void* x, const void* a, const void* b, const fl
     const LoraArgs p{x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status, T, K, N, E, R, S, n_seg};
     if (dtype == 0) return launch_general<float>(p, stream);
     if (!lora_mma_takes(p)) return launch_general<__nv_bfloat16>(p, stream);
-    const bool many = g_lora_form == 0 ? T >= LORA_TILE_TOKENS && T / n_seg >= LORA_TILE_SEGMENT &&
-                                             (long long)(T / 16) * 2 * R * ((long long)S * K + N) >= LORA_TILE_BYTES
-                                       : g_lora_form == 2;
+    const bool many = g_lora_form == 0 ? lora_many(p) : g_lora_form == 2;
     return many && lora_tiles_take(p) ? lora_tiles(p, fd_sm_count(), stream) : lora_rows(p, fd_sm_count(), stream);
 }

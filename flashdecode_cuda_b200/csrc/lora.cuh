@@ -95,13 +95,14 @@ __device__ __forceinline__ void lora_copy(const int* tok, int count, const void*
 }
 
 // The most tiles there can be: every segment ends with one that may not be full.
-inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (long long)p.T / rows + p.n_seg; }
+inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (p.T + (long long)(rows - 1) * p.n_seg) / rows; }
 
 // The kernels on the tensor cores (lora_mma.cu): whether they take the sizes, and the launch.
 bool lora_mma_takes(const LoraArgs& p);
 int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream);
 // ... and with tiles of 128 tokens (lora_tcgen05.cu): whether they take the sizes too, and the launch.
 bool lora_tiles_take(const LoraArgs& p);
+int lora_tile_cluster(const LoraArgs& p, int sms);
 int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream);
 
 }  // namespace fd

@@ -29,6 +29,9 @@ constexpr int LT_TILE = 128 * 128;               // bytes of a tile of 64 column
 constexpr int LT_Y_BYTES = 2 * LT_TILE;          // y's tile of 128 columns: two of those
 constexpr int LT_RING = 8, LT_OUT_RING = 3;      // most stages of step 1 and of step 3
 constexpr int LT_SMEM = 225 * 1024;
+// Clusters with an SM for each CTA that run at once; they have to lie within one of the GPU's groups of 16 to 18 SMs.  One more takes a second
+// wave: 13824 x 5120, rank 64, 15 tiles 36 us and 16 65 (in clusters of 4: 52), 33 tiles 56 us and 34 99 (in clusters of 2: 88).
+constexpr int LT_ROOM8 = 15, LT_ROOM4 = 33;
 constexpr int LT_MAX_W = 192;                    // columns of D1
 
 struct LoraTilePlan {
@@ -52,6 +55,17 @@ static LoraTilePlan lora_tile_plan(const LoraArgs& p) {
 }
 
 bool lora_tiles_take(const LoraArgs& p) { return lora_tile_plan(p).stages > 0; }
+
+// CTAs of a tile, by the tiles that there should be: T / 128, and a part of one for each segment's last.  One tile too many for a wave costs
+// some 15 to 20 % over clusters of half the size (34 tiles of 3584 x 3584, rank 32: 54 us, 45 in clusters of 2), clusters of half the size
+// where there was room cost 45 to 75 % (32 tiles: 45 us, 31 in clusters of 4), so a quarter of a tile is counted, not the half that
+// segments of any length leave empty.
+int lora_tile_cluster(const LoraArgs& p, int sms) {
+    const long long likely = std::min(lora_max_tiles(p, LT_ROWS), std::max<long long>((p.T + LT_ROWS - 1) / LT_ROWS, p.T / LT_ROWS + p.n_seg / 4));
+    int C = 8;
+    while (C > 1 && (likely > (C == 8 ? LT_ROOM8 : (C == 4 ? LT_ROOM4 : sms / C)) || (p.K + 63) / 64 < C)) C /= 2;
+    return C;
+}
 
 __device__ __forceinline__ uint32_t lt_swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
@@ -400,9 +414,7 @@ static int lora_map(CUtensorMap* map, const void* ptr, long long rows, int cols,
 int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream) {
     const LoraTilePlan f = lora_tile_plan(p);
     const long long tiles = lora_max_tiles(p, LT_ROWS);
-    // (clusters of 8 with an SM for each CTA find room two to a group of 16 to 18 SMs: 17 of them take two waves)
-    int C = tiles <= 16 ? 8 : 4;
-    while (C > 1 && (tiles * C > sms || (p.K + 63) / 64 < C)) C /= 2;
+    const int C = lora_tile_cluster(p, sms);
     FD_REQUIRE(tiles * C < (1ll << 31), -2, "lora_add: %d tokens", p.T);
     FD_REQUIRE((long long)p.E * p.N < (1ll << 31) && (long long)p.E * p.S * p.R < (1ll << 31), -2, "lora_add: %d adapters of %d rows", p.E, p.N);
     LoraMaps maps;
