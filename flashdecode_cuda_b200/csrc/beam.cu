@@ -12,6 +12,11 @@
 // CTA picks from there - one launch, no memory in between.  More: one kernel streams all rows with the whole GPU, a second one picks
 // (the clusters' other CTAs would hold their SMs while the first ones pick).
 //
+// What bounds it.  Many requests: the scan, by HBM.  64 requests of 8 rows of 152,064 (311 MB, floor 47.6 us) take 64.2 us: the scan 52 (6.0
+// TB/s), the pick 12 - a chain of a few dozen block-wide steps on 64 CTAs, which starts early (programmatic launch) but has nothing to do
+// before the last row's maxima are there.  Few requests: latency.  One request of 4 rows of 151,936 takes 12.2 us and seven of 3 to
+// 8 rows of 50,257 13.3, of which the bytes would be 0.4 and 1.1: launch and cluster start 3, streaming 160 KB per CTA 4, the pick 5.
+//
 // Why the sums are in 64 bits: which of two candidates of different beams comes first hangs on the difference of two
 // normalisers.  In 32 bits they are off by some 1e-6, and among the candidates of a large batch two that are nearer than
 // that are common (gaps of 1e-2 between neighbours: one pair in ten thousand, and a step of 64 requests has a thousand pairs).  The
@@ -36,6 +41,7 @@ constexpr int BM_BATCH = 4;              // such units that a warp has in flight
 constexpr int BM_SCAN_THREADS = 256, BM_SCAN_WARPS = BM_SCAN_THREADS / 32;
 constexpr int BM_PICK_THREADS = 1024;
 constexpr int BM_CLUSTER_THREADS = 512;
+constexpr int BM_WIDE = 14;              // clusters of 16 that run at once
 constexpr int BM_MAX_ROWS = 64;          // beams of one request
 constexpr int BM_MAX_K = 128;            // candidates of one request
 constexpr int BM_MAX_VOCAB = 1 << 22;    // so that the numbers of a request's groups and entries stay exact in 32 bits
@@ -545,10 +551,10 @@ beam_cluster_kernel(const float* __restrict__ logits, int V, int n, const float*
 
 using namespace fd;
 
-// Bytes of logits per CTA up to which the one launch is taken.  Measured, clusters / two kernels, us on the device and the host's time of a
-// call (11 / 15 us, the more of the two when calls follow each other): 4 rows of 151,936 (152 KB per CTA) 13.7 / 11.1; 36 ragged
-// rows of 50,257 for 7 requests (65 KB) 13.6 / 12.2; 106 rows of 2,410 for 53 8.7 / 9.5; but 3 requests of up to 28 rows of 82,102
-// (270 KB) 33 / 21, 512 rows of 152,064 for 64 95 / 65.
+// Bytes of logits per CTA up to which the one launch is taken.  Measured, clusters / two kernels, us on the device (a call costs the host 10
+// and 12 us, which is what counts when calls follow each other): 4 rows of 151,936 (152 KB per CTA) 12.4 / 11.3; 36 ragged rows of 50,257
+// for 7 requests (65 KB) 13.3 / 11.4; 64 rows of 32,000 for 16 10.6 / 10.0; 106 rows of 2,410 for 53 8.4 / 8.6; but 16 rows of 152,064 for one
+// request (608 KB) 34 / 20, 73 of 82,102 for 3 (500 KB) 42 / 25, 256 of 151,936 for 64 (608 KB) 53 / 39.
 constexpr long long BM_CLUSTER_BYTES = 160 * 1024;
 
 // Bytes of scratch that fd_beam_select needs for n rows of V logits (8-byte aligned).
@@ -580,8 +586,9 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     const bool small = V <= BM_SMALL_VOCAB;
     const bool vec = !small && V % 4 == 0 && (reinterpret_cast<unsigned long long>(logits) & 15) == 0;
     const int sms = fd_sm_count(), units = (V + BM_UNIT - 1) / BM_UNIT, size = small ? BM_SMALL_GROUP : BM_GROUP, groups = (V + size - 1) / size;
+    // (64 rows of 32,000 for 16 requests took 17.7 us in clusters of 16, of which 14 run at once, and take 10.6 in clusters of 8)
     int C = 16;
-    while (C > 1 && (R * C > 2 * sms || units < C)) C /= 2;
+    while (C > 1 && (R * C > 2 * sms || units < C || (C == 16 && R > BM_WIDE))) C /= 2;
     // (a request may have all the rows, up to 64)
     const long long smem = 4ll * (n < BM_MAX_ROWS ? n : BM_MAX_ROWS) * ((units + C - 1) / C) * (BM_UNIT / size);
     const bool fits = smem <= 96 * 1024 && R <= 2 * sms;

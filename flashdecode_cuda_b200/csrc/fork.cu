@@ -7,7 +7,10 @@
 //
 // Both move bytes and do nothing else: bound by HBM, half of the traffic reads and half writes.  A thread moves 16 bytes at a
 // time with several loads in flight before the first store; tensors whose rows are no multiple of that are moved in the largest
-// unit that divides them.
+// unit that divides them.  A CTA per copy and plane of blocks (per copy and 32 KB of states): a full server's copies are thousands of CTAs,
+// and one request's are a CTA per SM or two, whose time is the launch and two trips to memory.
+// Measured: 90 copies of up to 64 tokens in 96 planes of 8 heads of 128 (1.11 GB) 172.9 us, 6.44 TB/s, a plain copy's rate; 3 copies in 56
+// planes of 2 heads (6 MB) 2.8 us; 60 slots of 48 states (3.16 GB) 490 us, 6.45 TB/s; 3 slots of 12 states (10 MB) 3.4 us.
 #include "common.cuh"
 
 namespace fd {

@@ -11,6 +11,10 @@
 //      both); the epilogue takes each column from its own.  The tiles' y and B are a stage or two ahead.
 // One warp asks for copies, one thread issues MMAs, eight warps do the rest.  out takes y's place in shared memory, so that it leaves in
 // whole lines although a thread's share of D2 is a row.
+//
+// Measured: four prompts of 1,900 to 2,048 tokens, 13824 x 5120, rank 64 (390 MB, floor 59.7 us): 93 us, 4.2 TB/s - finding the tile 3, step 1 47
+// (an SM takes 57 GB/s, a third of it A, which every tile reads anew out of L2), step 2 5, step 3 32 (5.1 TB/s of y and out).  The two
+// streams follow one another, the exchange stands between them, and 65 tiles in clusters of 2 leave 18 SMs idle.  Tensor pipe 11 %.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -84,8 +88,8 @@ struct LoraMaps {
     CUtensorMap x[3], y[3], a, b;
 };
 
-// The rows of a tile's tokens: neighbours all of them (a prompt's tokens are), or 16 by 16, or gathered four by four, which the copy
-// engine does some ten times slower.
+// The rows of a tile's tokens: neighbours all of them (a prompt's tokens are), or 16 by 16, or gathered four by four: 32 copies of 512 bytes
+// for a tile's 64 columns instead of one of 16 KB, at some 85 cycles of the asking warp each.
 struct LoraRows {
     bool all;
     int first;               // of the tile
