@@ -217,7 +217,7 @@ static int launch_general(const LoraArgs& p, cudaStream_t stream) {
     const size_t smem = sizeof(float) * LR_ROWS * (chunk + (size_t)W + lora_sums(p.S, p.R));
     const long long tiles = lora_max_tiles(p, LR_ROWS);
     // where the tiles leave SMs idle, several clusters share a tile's columns (each computes the same A x)
-    int copies = (int)(2 * fd_sm_count() / (tiles * C));
+    int copies = (int)(lora_room(C, fd_sm_count()) / tiles);
     while (copies > 1 && p.N < LR_THREADS * C * copies) --copies;
     if (copies < 1) copies = 1;
     FD_REQUIRE(tiles * C * copies < (1ll << 31), -2, "lora_add: %d tokens", p.T);

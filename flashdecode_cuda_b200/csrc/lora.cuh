@@ -97,6 +97,9 @@ __device__ __forceinline__ void lora_copy(const int* tok, int count, const void*
 // The most tiles there can be: every segment ends with one that may not be full.
 inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (p.T + (long long)(rows - 1) * p.n_seg) / rows; }
 
+// Clusters of C CTAs, two CTAs to an SM, that run at once: a cluster lies within one of the GPU's groups of some 18 SMs.
+inline int lora_room(int C, int sms) { return C == 16 ? 14 : (C == 8 ? 33 : 2 * sms / C); }
+
 // The kernels on the tensor cores (lora_mma.cu): whether they take the sizes, and the launch.
 bool lora_mma_takes(const LoraArgs& p);
 int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream);

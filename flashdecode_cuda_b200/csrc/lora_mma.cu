@@ -17,6 +17,8 @@
 // (floor 6.6), bound by what the tiles read of A and B out of L2.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "lora.cuh"
 #include "mma_utils.cuh"
 
@@ -26,8 +28,6 @@ namespace cg = cooperative_groups;
 
 constexpr int LM_THREADS = 256, LM_WARPS = LM_THREADS / 32;
 constexpr int LM_ROWS = 16;              // tokens of a tile: the rows of an MMA
-constexpr int LM_CTAS = 2;               // per SM
-constexpr int LM_WIDE = 14;              // clusters of 16 that run at once
 constexpr int LM_TILES = 4;              // tiles of 8 rows of A that a warp accumulates at once
 constexpr int LM_RED = LM_TILES * 8 + 4; // floats of a token's row of a warp's sums (4: so that neighbouring rows are in other banks)
 
@@ -219,7 +219,7 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const __nv_bfloat
     }
 }
 
-__global__ void __launch_bounds__(LM_THREADS, LM_CTAS)
+__global__ void __launch_bounds__(LM_THREADS, 2)
 lora_rows_kernel(const LoraArgs p, int copies) {
     extern __shared__ __align__(16) unsigned char lm_smem[];
     cg::cluster_group cluster = cg::this_cluster();
@@ -373,14 +373,15 @@ bool lora_mma_takes(const LoraArgs& p) {
 int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream) {
     const long long tiles = lora_max_tiles(p, LM_ROWS);
     const int most = p.K > p.N ? p.K : p.N;
-    // Fourteen clusters of 16 run at once (groups of 16 or 18 SMs, two CTAs each); a fifteenth would double the time.  A segment's
-    // last tile is half full on average.
-    int C = p.n_seg <= LM_WIDE && p.T / LM_ROWS + (p.n_seg + 1) / 2 <= LM_WIDE ? 16 : 8;
-    while (C > 1 && (tiles * C > LM_CTAS * sms || most < 64 * C)) C /= 2;
-    // where that leaves SMs idle, several clusters share a tile's columns (and each computes A x: the second reads A from L2)
-    int copies = (int)(LM_CTAS * sms / (tiles * C));
+    // The largest cluster of which all run at once, by the tiles that there should be (T / 16, and a part of one for each segment's last), and
+    // where half of them would still run at once, several clusters share a tile's columns (and each computes A x: the second reads A from
+    // L2).  One cluster too many takes a second wave: 3584 x 37888 in two slices, rank 64, 8 tokens of 8 adapters in 16 clusters of 16 29
+    // us, in 8 22; 17 adapters in 34 clusters of 8 45, in 17 35.
+    const long long likely = std::min(tiles, std::max<long long>(p.n_seg, p.T / LM_ROWS + p.n_seg / 4));
+    int C = 16;
+    while (C > 1 && (likely > lora_room(C, sms) || most < 64 * C)) C /= 2;
+    int copies = std::max(1, (int)(lora_room(C, sms) / likely));
     while (copies > 1 && p.N < 256 * C * copies) --copies;
-    if (copies < 1) copies = 1;
     FD_REQUIRE(tiles * C * copies < (1ll << 31), -2, "lora_add: %d tokens", p.T);
     const int W = p.S * p.R;
     const size_t smem = sizeof(float) * (LM_WARPS * LM_ROWS * LM_RED + (size_t)LM_ROWS * W) + 2 * sizeof(__nv_bfloat16) * (size_t)LM_ROWS * lora_row_places(p.S, p.R);
