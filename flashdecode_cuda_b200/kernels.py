@@ -1749,7 +1749,8 @@ def lora_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Ten
              start: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None,
              col_slice: Optional[torch.Tensor] = None, slices: int = 1, status: Optional[torch.Tensor] = None) -> None:
     """out[t] = y[t] + scale[e] * b[e] (a[e] x[t]), e the adapter of token t: the low-rank terms of many requests at once, beside the
-    shared projection ``y`` [T, N] of ``x`` [T, K].  ``out`` may be ``y`` (and is when it is not given).
+    shared projection ``y`` [T, N] of ``x`` [T, K].  ``out`` may be ``y`` (and is when it is not given); it
+    shares no memory with ``x``, or with ``y`` other than being it.
 
     The tokens' adapters: ``order`` (int32 [T]) has every token once, sorted by adapter; the tokens order[start[i]:start[i + 1]] use
     the adapter ``ids[i]`` (-1: none, out[t] = y[t]); ``start`` int32 [segments + 1], ``ids`` int32 [segments].  Segments may be empty;
@@ -1777,6 +1778,7 @@ def lora_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Ten
     if not (col_slice is None or (col_slice.dtype is torch.uint8 and col_slice.numel() * 8 == N)):
         raise KernelError("lora_add: col_slice is uint8 [N / 8]")
     at = _pointers(x, a, b, scale, ranks, order, start, ids, y, out, col_slice, status)
-    if at[9] == at[0] and T:
-        raise KernelError("lora_add: out is x, which other tokens' products still read")
+    to, size = at[9], y.nbytes
+    if size and (at[0] < to + size and to < at[0] + x.nbytes or to != at[8] and at[8] < to + size and to < at[8] + size):
+        raise KernelError("lora_add: out is x, or shares memory with it or with a part of y, which other tokens still read")
     _check(lib().fd_lora_add(*at[:11], _dt(dt), T, Kd, N, E, R, slices, n_seg, at[11], _here_stream()))

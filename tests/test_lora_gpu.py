@@ -330,3 +330,57 @@ def test_an_output_over_the_input_is_refused():
     with pytest.raises(K.KernelError, match="out is x"):
         K.lora_add(x, torch.zeros(1, 4, 16, device=DEV), torch.zeros(1, 16, 4, device=DEV), torch.zeros(1, device=DEV), i(1), i(3), i(2), i(1),
                    torch.zeros(3, 16, device=DEV), x)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_an_output_that_shares_memory_in_part_is_refused(dtype):
+    dt = DT[dtype]
+    z, i = (lambda *s: torch.zeros(*s, device=DEV, dtype=dt)), (lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV))
+    both = z(7, 16)
+    call = lambda x, y, out: K.lora_add(x, z(1, 4, 16), z(1, 16, 4), torch.zeros(1, device=DEV), i(1), i(3), i(2), i(1), y, out)
+    for x, y, out in [(z(3, 16), both[:3], both[1:4]), (z(3, 16), both[1:4], both[:3]), (both[:3], z(3, 16), both[2:5]), (both[4:], both[2:5], both[2:5])]:
+        with pytest.raises(K.KernelError, match="shares memory"):
+            call(x, y, out)
+    both.fill_(2.0)
+    call(both[:3], both[3:6], both[3:6])                         # neighbours share nothing
+    call(z(3, 16), both[:3], both[3:6])
+    assert bool((both == 2).all())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("E", [7, 8, 14, 15, 17, 33, 34])
+def test_one_token_of_each_of_many_adapters(dtype, E):
+    # one token to a tile, as many clusters as run at once and one more
+    check(dtype, E, 1024, 2056, E, 8, token=list(range(E)))
+    check(dtype, E, 4096, 520, E, 16, token=list(range(E)), in_place=True)
+
+
+@pytest.mark.parametrize("T", [15 * 128, 15 * 128 + 1, 33 * 128, 33 * 128 + 1])
+def test_as_many_large_tiles_as_run_at_once_and_one_more(T):
+    K.lora_set_form(2)
+    try:
+        check("bfloat16", T, 520, 136, 1, 8, token=[0] * T)
+        check("bfloat16", T, 520, 136, 3, 8, token=[min(t * 4 // T, 2) for t in range(T)], in_place=True, seed=2)
+    finally:
+        K.lora_set_form(0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("N", [1, 7, 8, 12, 136, 4872])
+@pytest.mark.parametrize("form", [1, 2])
+def test_rows_without_an_adapter_come_out_as_they_are(dtype, N, form):
+    # every token but a few, here and there; rows on and off the 16-byte boundary; an adapter of rank zero with a scale that is no number
+    T, Kd, R = 413, 64, 8
+    for off in (0, 1):
+        g = torch.Generator().manual_seed(N + off)
+        y = torch.randn(T * N + off, generator=g).to(DT[dtype]).to(DEV)[off:].view(T, N)
+        out = torch.full((T * N + off,), 9.0, dtype=DT[dtype], device=DEV)[off:].view(T, N)
+        token = torch.randint(-1, 2, (T,), generator=g).tolist()
+        x = torch.randn(T, Kd, generator=g).to(DT[dtype]).to(DEV)
+        K.lora_set_form(form)
+        try:
+            K.lora_add(x, torch.zeros(2, R, Kd, dtype=DT[dtype], device=DEV), torch.zeros(2, N, R, dtype=DT[dtype], device=DEV),
+                       torch.tensor([1.0, float("inf")], device=DEV), torch.tensor([R, 0], dtype=torch.int32, device=DEV), *plan(token), y, out)
+        finally:
+            K.lora_set_form(0)
+        assert torch.equal(out, y)
