@@ -12,10 +12,10 @@
 // CTA picks from there - one launch, no memory in between.  More: one kernel streams all rows with the whole GPU, a second one picks
 // (the clusters' other CTAs would hold their SMs while the first ones pick).
 //
-// What bounds it.  Many requests: the scan, by HBM.  64 requests of 8 rows of 152,064 (311 MB, floor 47.6 us) take 64.2 us: the scan 52 (6.0
-// TB/s), the pick 12 - a chain of a few dozen block-wide steps on 64 CTAs, which starts early (programmatic launch) but has nothing to do
-// before the last row's maxima are there.  Few requests: latency.  One request of 4 rows of 151,936 takes 12.2 us and seven of 3 to
-// 8 rows of 50,257 13.3, of which the bytes would be 0.4 and 1.1: launch and cluster start 3, streaming 160 KB per CTA 4, the pick 5.
+// What bounds it.  Many requests: the scan, by HBM.  64 requests of 8 rows of 152,064 (311 MB, floor 47.6 us) take 62.8 us: the scan 52 (6.0
+// TB/s), the pick 11 - a chain of a few dozen block-wide steps on 64 CTAs, which starts early (programmatic launch) but has nothing to do
+// before the last row's maxima are there.  Few requests: latency.  One request of 4 rows of 151,936 takes 12 us and seven of 3 to
+// 8 rows of 50,257 13, of which the bytes would be 0.4 and 1.1: launch and cluster start 3, streaming 160 KB per CTA 4, the pick 5.
 //
 // Why the sums are in 64 bits: which of two candidates of different beams comes first hangs on the difference of two
 // normalisers.  In 32 bits they are off by some 1e-6, and among the candidates of a large batch two that are nearer than
@@ -25,6 +25,7 @@
 // no common sign and average out over the row.  Groups of 16 are added in 32 bits, then in 64.
 #include <cooperative_groups.h>
 #include <math.h>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -251,6 +252,7 @@ struct BeamShared {
     int fidx[BM_FOUND], idx[BM_KEPT];
     int list[BM_LIST];
     int scratch[33];
+    int counts[2][32];
     int n_list, n_found, n_kept;
 };
 struct BeamOut {
@@ -306,13 +308,21 @@ __device__ __forceinline__ double2 beam_offset(float score, int pieces, Piece pi
 }
 
 // A number that at least k of the threads' `keys` (N of them each, 0: none) reach, and hardly more; 1 where there are fewer than k.
-template <int N>
-__device__ __forceinline__ unsigned long long beam_threshold(const unsigned long long (&keys)[N], int k) {
+template <int THREADS, int N>
+__device__ __forceinline__ unsigned long long beam_threshold(BeamShared& sh, const unsigned long long (&keys)[N], int k) {
+    constexpr int WARPS = THREADS / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int step = 0;
     auto reach = [&](unsigned long long q) {
+        if constexpr (N == 1) return __syncthreads_count(keys[0] >= q);
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) c += __syncthreads_count(keys[i] >= q);
-        return c;
+        for (int i = 0; i < N; ++i) c += keys[i] >= q;
+        c = __reduce_add_sync(0xffffffffu, c);
+        int* to = sh.counts[step++ & 1];                         // (the one before is still being read)
+        if (lane == 0) to[warp] = c;
+        __syncthreads();
+        return __reduce_add_sync(0xffffffffu, lane < WARPS ? to[lane] : 0);
     };
     if (reach(1ull) < k) return 1ull;
     unsigned long long T = 0ull;
@@ -351,7 +361,7 @@ __device__ void beam_pick(BeamShared& sh, const float* __restrict__ x, int V, in
         where = more ? i : where;
         mine[0] = more ? q : mine[0];
     }
-    unsigned long long T = beam_threshold(mine, k);
+    unsigned long long T = beam_threshold<THREADS>(sh, mine, k);
     auto list = [&](int i) {
         const int p = atomicAdd(&sh.n_list, 1);
         if (p < BM_LIST) sh.list[p] = i;
@@ -366,22 +376,35 @@ __device__ void beam_pick(BeamShared& sh, const float* __restrict__ x, int V, in
     int ng = sh.n_list;
     const bool listed = ng <= BM_LIST;
     constexpr int EACH = GROUP / 32;                             // entries of a group per lane
-    if (listed) {
-        for (int j = warp; j < ng; j += WARPS) {
-            const int i = sh.list[j], b = maxima.row(i), v0 = (i - b * groups) * GROUP;
-            float e[EACH];
+    // `many`: groups that a warp reads at once
+    auto read = [&](auto many) {
+        constexpr int BATCH = decltype(many)::value;
+        for (int j0 = warp; j0 < ng; j0 += WARPS * BATCH) {
+            float e[BATCH][EACH];
+            int row[BATCH], at0[BATCH];
 #pragma unroll
-            for (int u = 0; u < EACH; ++u) e[u] = v0 + u * 32 + lane < V ? __ldg(x + (size_t)b * V + v0 + u * 32 + lane) : -INFINITY;
+            for (int c = 0; c < BATCH; ++c) {
+                const int i = sh.list[min(j0 + c * WARPS, ng - 1)];
+                row[c] = maxima.row(i);
+                at0[c] = (i - row[c] * groups) * GROUP + lane;
 #pragma unroll
-            for (int u = 0; u < EACH; ++u) {
-                const unsigned long long q = beam_key(sh.off[b], e[u]);
-                if (q >= T) {
-                    const int p = atomicAdd(&sh.n_found, 1);
-                    if (p < BM_FOUND) { sh.fkey[p] = q; sh.fidx[p] = b * V + v0 + u * 32 + lane; }
-                }
+                for (int u = 0; u < EACH; ++u)
+                    e[c][u] = j0 + c * WARPS < ng && at0[c] + u * 32 < V ? __ldg(x + (size_t)row[c] * V + at0[c] + u * 32) : -INFINITY;
             }
+#pragma unroll
+            for (int c = 0; c < BATCH; ++c)
+#pragma unroll
+                for (int u = 0; u < EACH; ++u) {
+                    const unsigned long long q = beam_key(sh.off[row[c]], e[c][u]);
+                    if (q >= T) {                                // (T is 1 or more: not what is no candidate)
+                        const int p = atomicAdd(&sh.n_found, 1);
+                        if (p < BM_FOUND) { sh.fkey[p] = q; sh.fidx[p] = row[c] * V + at0[c] + u * 32; }
+                    }
+                }
         }
-    }
+    };
+    if (listed && ng <= WARPS) read(std::integral_constant<int, 1>());
+    else if (listed) read(std::integral_constant<int, EACH == 1 ? 4 : 2>());
     __syncthreads();
     const unsigned long long* key = sh.fkey;
     const int* idx = sh.fidx;
@@ -392,7 +415,7 @@ __device__ void beam_pick(BeamShared& sh, const float* __restrict__ x, int V, in
         unsigned long long own[BM_FOUND / THREADS];
 #pragma unroll
         for (int u = 0; u < BM_FOUND / THREADS; ++u) own[u] = t + u * THREADS < nf ? sh.fkey[t + u * THREADS] : 0ull;
-        const unsigned long long T2 = beam_threshold(own, k);
+        const unsigned long long T2 = beam_threshold<THREADS>(sh, own, k);
 #pragma unroll
         for (int u = 0; u < BM_FOUND / THREADS; ++u)
             if (own[u] >= T2 && own[u] != 0ull) {
@@ -454,17 +477,19 @@ __device__ void beam_pick(BeamShared& sh, const float* __restrict__ x, int V, in
         idx = sh.idx;
         nf = sh.n_kept;
     }
-    // an entry's place is the number of entries before it
-    for (int j = t; j < nf; j += THREADS) {
+    // an entry's place is the number of entries before it: a warp counts them for one
+    for (int j = warp; j < nf; j += WARPS) {
         const unsigned long long q = key[j];
         const int id = idx[j];
-        int rank = 0;
-        for (int i = 0; i < nf; ++i) {
+        int before = 0;
+#pragma unroll 2
+        for (int i = lane; i < nf; i += 32) {
             const unsigned long long o = key[i];
-            rank += o > q || (o == q && idx[i] < id);
+            before += o > q || (o == q && idx[i] < id);
         }
-        if (rank < k) {
-            const size_t p = (size_t)r * k + rank;
+        const int place = __reduce_add_sync(0xffffffffu, before);
+        if (lane == 0 && place < k) {
+            const size_t p = (size_t)r * k + place;
             out.score[p] = (float)beam_value(q);
             out.row[p] = first + id / V;
             out.tok[p] = id % V;
@@ -551,11 +576,13 @@ beam_cluster_kernel(const float* __restrict__ logits, int V, int n, const float*
 
 using namespace fd;
 
-// Bytes of logits per CTA up to which the one launch is taken.  Measured, clusters / two kernels, us on the device (a call costs the host 10
-// and 12 us, which is what counts when calls follow each other): 4 rows of 151,936 (152 KB per CTA) 12.4 / 11.3; 36 ragged rows of 50,257
-// for 7 requests (65 KB) 13.3 / 11.4; 64 rows of 32,000 for 16 10.6 / 10.0; 106 rows of 2,410 for 53 8.4 / 8.6; but 16 rows of 152,064 for one
-// request (608 KB) 34 / 20, 73 of 82,102 for 3 (500 KB) 42 / 25, 256 of 151,936 for 64 (608 KB) 53 / 39.
+// Bytes of logits per CTA, and rows per request, up to which the one launch is taken.  Measured, clusters / two kernels, us on the device (a
+// call costs the host 10 to 13 and 12 to 17 us, which is what counts when calls follow each other): 4 rows of 151,936 (152 KB per CTA)
+// 12.1 / 10.4; 36 ragged rows of 50,257 for 7 requests (65 KB) 13.1 / 10.6; 64 rows of 32,000 for 16 10.1 / 9.5; 106 rows of 2,410 for 53
+// 8.2 / 8.4; but 117 of 120,971 for 13 (272 KB) 31 / 22, 512 of 152,064 for 64 93 / 63; 22 rows of 14,151 for one request 21 / 14.5, 240
+// of 1,000 for 8 15.8 / 11.6: many rows have many maxima, and of the two picks the one of 1,024 threads that reads them from L2 is the faster.
 constexpr long long BM_CLUSTER_BYTES = 160 * 1024;
+constexpr int BM_CLUSTER_ROWS = 12;
 
 // Bytes of scratch that fd_beam_select needs for n rows of V logits (8-byte aligned).
 extern "C" long long fd_beam_select_scratch_bytes(int n, int V) {
@@ -592,7 +619,7 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     // (a request may have all the rows, up to 64)
     const long long smem = 4ll * (n < BM_MAX_ROWS ? n : BM_MAX_ROWS) * ((units + C - 1) / C) * (BM_UNIT / size);
     const bool fits = smem <= 96 * 1024 && R <= 2 * sms;
-    if (fits && g_beam_form != 2 && (g_beam_form == 1 || 4ll * n * V <= BM_CLUSTER_BYTES * R * C)) {
+    if (fits && g_beam_form != 2 && (g_beam_form == 1 || (n <= BM_CLUSTER_ROWS * R && 4ll * n * V <= BM_CLUSTER_BYTES * R * C))) {
         const int which = small ? 2 : (vec ? 1 : 0);
         void (*const kernels[3])(const float*, int, int, const float*, const int*, int, int, int, const BeamOut, int*) = {
             beam_cluster_kernel<false, false>, beam_cluster_kernel<true, false>, beam_cluster_kernel<false, true>};
