@@ -294,3 +294,21 @@ def test_largest_vocabulary_and_beyond():
     check(x, torch.zeros(2), [0, 2], 4)
     with pytest.raises(K.KernelError, match="vocabulary"):
         select(torch.zeros(1, K.BEAM_MAX_VOCAB + 1), torch.zeros(1), [0, 1], 4)
+
+
+@pytest.mark.parametrize("form", [1, 2])
+@pytest.mark.parametrize("V,beams,k", [(335, [26, 25], 53), (1191, [29, 3, 64], 59), (14151, [22], 55), (16384, [40], 128), (16385, [30], 64), (324, [10] * 5, 21), (40000, [12, 13], 128)])
+def test_many_rows_of_nearly_the_same_score(form, V, beams, k):
+    # the best come from all rows: groups of many rows to read again, and more entries than are ranked at once
+    K.beam_select_set_form(form)
+    try:
+        g = torch.Generator().manual_seed(V + 7 * k)
+        start = [0]
+        for b in beams:
+            start.append(start[-1] + b)
+        n = start[-1]
+        x, scores = torch.randn(n, V, generator=g), 0.1 * torch.rand(n, generator=g)
+        check(x, scores, start, k)
+        check(torch.round(2.0 * x) / 2.0, scores, start, k)          # ties within every row
+    finally:
+        K.beam_select_set_form(0)
