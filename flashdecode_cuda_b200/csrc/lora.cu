@@ -48,7 +48,7 @@ __host__ __device__ __forceinline__ int lora_sums(int S, int R) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LR_THREADS)
+__global__ void __launch_bounds__(LR_THREADS, 2)
 lora_general_kernel(const LoraArgs p, int copies, int chunk) {
     extern __shared__ __align__(16) float lr_smem[];
     cg::cluster_group cluster = cg::this_cluster();
@@ -220,7 +220,7 @@ static int launch_general(const LoraArgs& p, cudaStream_t stream) {
     const size_t smem = sizeof(float) * LR_ROWS * (chunk + (size_t)W + lora_sums(p.S, p.R));
     const long long tiles = lora_max_tiles(p, LR_ROWS);
     // where the tiles leave SMs idle, several clusters share a tile's columns (each computes the same A x)
-    int copies = (int)(lora_room(C, fd_sm_count()) / tiles);
+    int copies = (int)(lora_room(C, fd_sm_count()) / lora_likely_tiles(p));
     while (copies > 1 && p.N < LR_THREADS * C * copies) --copies;
     if (copies < 1) copies = 1;
     FD_REQUIRE(tiles * C * copies < (1ll << 31), -2, "lora_add: %d tokens", p.T);

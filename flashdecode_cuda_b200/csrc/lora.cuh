@@ -97,6 +97,12 @@ __device__ __forceinline__ void lora_copy(const int* tok, int count, const void*
 // The most tiles there can be: every segment ends with one that may not be full.
 inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (p.T + (long long)(rows - 1) * p.n_seg) / rows; }
 
+// Tiles of 16 tokens that there should be: T / 16, and a part of one for each segment's last; of single tokens one each.
+inline long long lora_likely_tiles(const LoraArgs& p) {
+    const long long most = lora_max_tiles(p, 16), some = (long long)p.T / 16 + p.n_seg / 4;
+    return most < p.n_seg || most < some ? most : (some > p.n_seg ? some : p.n_seg);
+}
+
 // Clusters of C CTAs, two CTAs to an SM, that run at once: a cluster lies within one of the GPU's groups of some 18 SMs.
 inline int lora_room(int C, int sms) { return C == 16 ? 14 : (C == 8 ? 33 : 2 * sms / C); }
 

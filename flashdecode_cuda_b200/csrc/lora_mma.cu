@@ -373,11 +373,11 @@ bool lora_mma_takes(const LoraArgs& p) {
 int lora_rows(const LoraArgs& p, int sms, cudaStream_t stream) {
     const long long tiles = lora_max_tiles(p, LM_ROWS);
     const int most = p.K > p.N ? p.K : p.N;
-    // The largest cluster of which all run at once, by the tiles that there should be (T / 16, and a part of one for each segment's last), and
+    // The largest cluster of which all run at once, by the tiles that there should be, and
     // where half of them would still run at once, several clusters share a tile's columns (and each computes A x: the second reads A from
     // L2).  One cluster too many takes a second wave: 3584 x 37888 in two slices, rank 64, 8 tokens of 8 adapters in 16 clusters of 16 29
     // us, in 8 22; 17 adapters in 34 clusters of 8 45, in 17 35.
-    const long long likely = std::min(tiles, std::max<long long>(p.n_seg, p.T / LM_ROWS + p.n_seg / 4));
+    const long long likely = lora_likely_tiles(p);
     int C = 16;
     while (C > 1 && (likely > lora_room(C, sms) || most < 64 * C)) C /= 2;
     int copies = std::max(1, (int)(lora_room(C, sms) / likely));

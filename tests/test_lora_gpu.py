@@ -384,3 +384,14 @@ def test_rows_without_an_adapter_come_out_as_they_are(dtype, N, form):
         finally:
             K.lora_set_form(0)
         assert torch.equal(out, y)
+
+
+@pytest.mark.parametrize("Kd,N,R,S", [(1536, 512, 16, 1), (4100, 304, 12, 2), (260, 100, 33, 1), (600, 1030, 4, 1), (96, 300, 8, 1)])
+def test_a_float32_token_has_the_same_bits_in_any_step(Kd, N, R, S):
+    T = 1300
+    d, cols, S = make("float32", T, Kd, N, 3, R, S)
+    token = [(t * 5) % 4 - 1 for t in range(T)]
+    want = run(d, cols, S, token)
+    for some in ([0], [5, 1299, 700], list(range(3, 560)), list(range(0, 1300, 2))):
+        part = dict(d, x=d["x"][some], y=d["y"][some])
+        assert torch.equal(run(part, cols, S, [token[t] for t in some]), want[some])
