@@ -76,14 +76,16 @@ template <typename U>
 __device__ __forceinline__ void lora_copy(const int* tok, int count, const void* from, void* to, int units, int u0, int u1, int t, int threads) {
     const U* f = static_cast<const U*>(from);
     U* o = static_cast<U*>(to);
-    const int width = u1 - u0, total = width > 0 ? width * count : 0;
-    for (int i0 = t; i0 < total; i0 += threads * 8) {
+    // (rows of up to 2^27 units, 16 of them, or of 2^24, 128: numbers of up to 2^31)
+    const unsigned width = u1 > u0 ? u1 - u0 : 0, total = width * count;
+    for (unsigned i0 = t; i0 < total; i0 += threads * 8) {
         U v[8];
         size_t at[8];
         bool here[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int i = i0 + j * threads, row = i / width, token = i < total ? tok[row] : -1;
+            const unsigned i = i0 + j * threads, row = i / width;
+            const int token = i < total ? tok[row] : -1;
             here[j] = token >= 0;
             at[j] = here[j] ? (size_t)token * units + u0 + (i - row * width) : 0;
             if (here[j]) v[j] = f[at[j]];
