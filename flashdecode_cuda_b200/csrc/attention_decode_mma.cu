@@ -41,7 +41,7 @@ static int launch_dm(const AttnParams& p, int n_rows, cudaStream_t stream) {
         configured = true;
     }
     dim3 grid(p.n_splits, p.n_kv, n_rows);
-    return launch("attention_decode_mma", k, grid, dim3(W * 32), smem, stream, dim3(1, 1, 1), p);
+    return launch_waiting("attention_decode_mma", k, grid, dim3(W * 32), smem, stream, dim3(1, 1, 1), p);
 }
 
 int g_dm_form = 0;       // tests and measurements: 0 = the launcher chooses; bit 0: heads as rows even for small groups;

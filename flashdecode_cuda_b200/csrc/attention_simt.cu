@@ -606,7 +606,7 @@ static int attention_impl(const void* q, const void* k_pool, const void* v_pool,
         if (use_mma != 0) rc = launch_attn_f32(one, n_rows, 1, stream);
         if (rc == 1) rc = launch_attn<float>(one, n_rows, 1, stream);
         if (rc == 0 && one.n_splits > 1)
-            rc = launch("attention_combine", attn_combine_kernel<float, true>, dim3(n_q, n_rows), dim3(128), 0, stream, dim3(1, 1, 1),
+            rc = launch_waiting("attention_combine", attn_combine_kernel<float, true>, dim3(n_q, n_rows), dim3(128), 0, stream, dim3(1, 1, 1),
                         (const float*)one.part_m, (const float*)one.part_l, (const float*)one.part_acc, (float*)out, tok_row,
                         row_slot, n_q, dv, one.n_splits, (const float*)nullptr, 1, 0, p.out_ld, out_scale, row_q_start, row_q_len);
         if (rc != 0) return rc;
@@ -638,11 +638,11 @@ static int attention_impl(const void* q, const void* k_pool, const void* v_pool,
     if (rc != 0 || n_splits == 1) return rc;
     dim3 grid(n_q * v_rep, T);
     if (dtype == 0)
-        return launch("attention_combine", attn_combine_kernel<float>, grid, dim3(128), 0, stream, dim3(1, 1, 1),
+        return launch_waiting("attention_combine", attn_combine_kernel<float>, grid, dim3(128), 0, stream, dim3(1, 1, 1),
                       (const float*)p.part_m, (const float*)p.part_l, (const float*)p.part_acc, (float*)out, tok_row,
                       row_slot, n_q * v_rep, dv, n_splits, sink, v_rep, out_f32, p.out_ld, out_scale, (const int*)nullptr,
                       (const int*)nullptr);
-    return launch("attention_combine", attn_combine_kernel<bf16>, grid, dim3(128), 0, stream, dim3(1, 1, 1),
+    return launch_waiting("attention_combine", attn_combine_kernel<bf16>, grid, dim3(128), 0, stream, dim3(1, 1, 1),
                   (const float*)p.part_m, (const float*)p.part_l, (const float*)p.part_acc, (bf16*)out, tok_row,
                   row_slot, n_q * v_rep, dv, n_splits, sink, v_rep, out_f32, p.out_ld, out_scale, (const int*)nullptr,
                   (const int*)nullptr);

@@ -92,12 +92,13 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 
 namespace fd {
 
-// Programmatic dependent launch.  A kernel launched through fd::launch may begin while the
+// Programmatic dependent launch.  A kernel launched through fd::launch_with or fd::launch_waiting may begin while the
 // kernel before it in the stream is still running: it calls pdl_launch_dependents() at its
 // top (so the one after it can be set up early too), does what depends on nothing written by
 // earlier kernels (fetching weights), and calls pdl_wait() before it first touches anything an
 // earlier kernel wrote or still reads.  pdl_wait() returns once every earlier kernel has
 // completed and its writes are visible.  Without the launch attribute both are no-ops.
+// A kernel that does not wait goes through fd::launch, whose launches never have the attribute.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -165,10 +166,16 @@ inline int launch_with(bool pdl, const char* what, void (*kernel)(KArgs...), dim
     return 0;
 }
 
-// The same, programmatic only while that is switched on for every kernel (fd_set_pdl; off by default).
+// A kernel that begins when the one before it has completed.
 template <typename... KArgs, typename... Args>
 inline int launch(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                   dim3 cluster, Args... args) {
+    return launch_with(false, what, kernel, grid, block, smem, stream, cluster, args...);
+}
+// A kernel that calls pdl_wait: programmatic only while that is switched on for these (fd_set_pdl; off by default).
+template <typename... KArgs, typename... Args>
+inline int launch_waiting(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                          dim3 cluster, Args... args) {
     return launch_with(g_pdl != 0, what, kernel, grid, block, smem, stream, cluster, args...);
 }
 

@@ -130,9 +130,9 @@ extern "C" int fd_add_dyn_tanh(const void* delta, int delta_dtype, float* resid,
 #define FD_DT(TD_, TO_)                                                                                             \
     do {                                                                                                            \
         if (vec)                                                                                                    \
-            return launch("add_dyn_tanh", add_dyn_tanh_kernel<TD_, TO_, true>, grid, dim3(DT_THREADS), 0, stream,  \
+            return launch_waiting("add_dyn_tanh", add_dyn_tanh_kernel<TD_, TO_, true>, grid, dim3(DT_THREADS), 0, stream,  \
                           dim3(1, 1, 1), (const TD_*)delta, resid, write_resid, w, b, alpha, (TO_*)out, rows, H);   \
-        return launch("add_dyn_tanh", add_dyn_tanh_kernel<TD_, TO_, false>, grid, dim3(DT_THREADS), 0, stream,     \
+        return launch_waiting("add_dyn_tanh", add_dyn_tanh_kernel<TD_, TO_, false>, grid, dim3(DT_THREADS), 0, stream,     \
                       dim3(1, 1, 1), (const TD_*)delta, resid, write_resid, w, b, alpha, (TO_*)out, rows, H);       \
     } while (0)
     if (out_dtype == 0) {

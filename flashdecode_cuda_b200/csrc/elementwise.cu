@@ -348,9 +348,9 @@ extern "C" int fd_embed(const int* tokens, const void* table, int table_dtype, f
     FD_REQUIRE(H > 0 && V > 0 && copies >= 1, -2, "embed: bad sizes H=%d V=%d copies=%d", H, V, copies);
     const int threads = H >= 1024 ? 256 : 128;
     if (table_dtype == 0)
-        return launch("embed", embed_kernel<float>, dim3(T), dim3(threads), 0, stream, dim3(1, 1, 1), tokens,
+        return launch_waiting("embed", embed_kernel<float>, dim3(T), dim3(threads), 0, stream, dim3(1, 1, 1), tokens,
                       (const float*)table, resid, H, V, copies, scale, status);
-    return launch("embed", embed_kernel<bf16>, dim3(T), dim3(threads), 0, stream, dim3(1, 1, 1), tokens,
+    return launch_waiting("embed", embed_kernel<bf16>, dim3(T), dim3(threads), 0, stream, dim3(1, 1, 1), tokens,
                   (const bf16*)table, resid, H, V, copies, scale, status);
 }
 
@@ -364,12 +364,12 @@ static int launch_norm(const void* delta, int n_parts, size_t part_stride, float
     if (w_dtype == 0) {
         auto k = add_rmsnorm_kernel<TD, float, TO>;
         if (smem > 48 * 1024) cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        return launch("add_rmsnorm", k, dim3(n_out), dim3(threads), smem, stream, dim3(1, 1, 1), (const TD*)delta, n_parts,
+        return launch_waiting("add_rmsnorm", k, dim3(n_out), dim3(threads), smem, stream, dim3(1, 1, 1), (const TD*)delta, n_parts,
                       part_stride, resid, write_resid, (const float*)w, eps, (TO*)out, rows, H, dscale);
     } else {
         auto k = add_rmsnorm_kernel<TD, bf16, TO>;
         if (smem > 48 * 1024) cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        return launch("add_rmsnorm", k, dim3(n_out), dim3(threads), smem, stream, dim3(1, 1, 1), (const TD*)delta, n_parts,
+        return launch_waiting("add_rmsnorm", k, dim3(n_out), dim3(threads), smem, stream, dim3(1, 1, 1), (const TD*)delta, n_parts,
                       part_stride, resid, write_resid, (const bf16*)w, eps, (TO*)out, rows, H, dscale);
     }
 }
@@ -404,15 +404,15 @@ int fd::add_rmsnorm(const void* delta, int delta_dtype, int n_parts, long long p
         const int threads = ((H / 8 + 31) / 32) * 32;
         if (n_parts <= 4) {
             if (w_dtype == 0)
-                return launch("add_rmsnorm", add_rmsnorm_row_parts_kernel<float, 4>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
+                return launch_waiting("add_rmsnorm", add_rmsnorm_row_parts_kernel<float, 4>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
                               (const float*)delta, n_parts, ps, resid, write_resid, (const float*)weight, eps, (bf16*)out, rows, H, dscale);
-            return launch("add_rmsnorm", add_rmsnorm_row_parts_kernel<bf16, 4>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
+            return launch_waiting("add_rmsnorm", add_rmsnorm_row_parts_kernel<bf16, 4>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
                           (const float*)delta, n_parts, ps, resid, write_resid, (const bf16*)weight, eps, (bf16*)out, rows, H, dscale);
         }
         if (w_dtype == 0)
-            return launch("add_rmsnorm", add_rmsnorm_row_parts_kernel<float, 8>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
+            return launch_waiting("add_rmsnorm", add_rmsnorm_row_parts_kernel<float, 8>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
                           (const float*)delta, n_parts, ps, resid, write_resid, (const float*)weight, eps, (bf16*)out, rows, H, dscale);
-        return launch("add_rmsnorm", add_rmsnorm_row_parts_kernel<bf16, 8>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
+        return launch_waiting("add_rmsnorm", add_rmsnorm_row_parts_kernel<bf16, 8>, dim3(n_out), dim3(threads), 0, stream, dim3(1, 1, 1),
                       (const float*)delta, n_parts, ps, resid, write_resid, (const bf16*)weight, eps, (bf16*)out, rows, H, dscale);
     }
     if (delta_dtype == 0 && out_dtype == 0)

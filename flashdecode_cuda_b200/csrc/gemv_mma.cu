@@ -184,15 +184,15 @@ static int launch_gemv(const GemvParams& p, const RopeArgs& ra, cudaStream_t str
     dim3 grid((p.N + rows - 1) / rows, p.n_splits);
     if (p.mode == 4) {
         if (p.n_splits > 1)
-            return launch("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, true, W, true>, grid, dim3(W * 32), 0, stream,
+            return launch_waiting("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, true, W, true>, grid, dim3(W * 32), 0, stream,
                           dim3(1, p.n_splits, 1), p, ra);
-        return launch("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, false, W, true>, grid, dim3(W * 32), 0, stream,
+        return launch_waiting("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, false, W, true>, grid, dim3(W * 32), 0, stream,
                       dim3(1, 1, 1), p, ra);
     }
     if (p.n_splits > 1 && p.mode != 0)
-        return launch("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, true, W, false>, grid, dim3(W * 32), 0, stream,
+        return launch_waiting("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, true, W, false>, grid, dim3(W * 32), 0, stream,
                       dim3(1, p.n_splits, 1), p, ra);
-    return launch("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, false, W, false>, grid, dim3(W * 32), 0, stream,
+    return launch_waiting("gemv_mma", gemv_mma_kernel<NT, WK, UNROLL, false, W, false>, grid, dim3(W * 32), 0, stream,
                   dim3(1, 1, 1), p, ra);
 }
 

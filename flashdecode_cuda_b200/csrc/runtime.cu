@@ -54,7 +54,7 @@ extern "C" int fd_sm_count() {
 // fd::check_launch), captured launches included: one count per launch call, not per replay of a graph.
 extern "C" unsigned long long fd_launch_count() { return fd::g_launches; }
 
-// Turn programmatic dependent launch on (1) or off (0, the default) for later launches.
+// Turn programmatic dependent launch on (1) or off (0, the default) for later launches of the kernels that wait for the one before them.
 extern "C" int fd_set_pdl(int on) {
     fd::g_pdl = on ? 1 : 0;
     return 0;
