@@ -594,12 +594,8 @@ static int launch_gs(const void* x, const void* w, GsParams& p, const TcRope& ra
         if (rc != 0) return rc;
     }
     g_gs_last_map3d = p.map3d;
-    const int pdl_before = g_pdl;
-    g_pdl = g_pdl || g_gs_pdl;
-    const int rc = launch_waiting(what, gemm_stream_tcgen05_kernel, dim3(pl.grid), dim3(GS_THREADS), pl.smem, stream, dim3(pl.splits, 1, 1),
-                          mw, mx, p, ra);
-    g_pdl = pdl_before;
-    return rc;
+    return launch_with(g_pdl != 0 || g_gs_pdl != 0, what, gemm_stream_tcgen05_kernel, dim3(pl.grid), dim3(GS_THREADS), pl.smem, stream,
+                       dim3(pl.splits, 1, 1), mw, mx, p, ra);
 }
 
 }  // namespace fd

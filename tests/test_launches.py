@@ -59,3 +59,11 @@ def test_the_plain_launch_never_begins_early():
     launch = block(text, text.index("inline int launch("))
     assert "launch_with(false" in launch
     assert "g_pdl" in block(text, text.index("inline int launch_waiting("))
+
+
+def test_a_launch_does_not_change_the_switch_for_others():
+    """Launches of several threads at once: the switch is written where it is set, and nowhere for the length of a launch."""
+    for name, text in sources().items():
+        text = text.replace("extern int g_pdl", "").replace("int g_pdl = 0;", "")
+        for m in re.finditer(r"\bg_pdl\s*=(?!=)", text):
+            assert name == "runtime.cu" and "fd_set_pdl" in text[:m.start()][-120:], f"{name} sets g_pdl"
