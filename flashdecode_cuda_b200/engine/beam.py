@@ -5,8 +5,9 @@ davidjoyme/flashdecode-cuda decodes one greedy sequence per row (engine/model.py
 request over its beams and the vocabulary are selected on the device (``kernels.beam_select``), and the beams that go on take over the
 cached keys, values and states of the ones they continue (``PagedCache.reorder``).  Only the selected candidates come to the host.
 
-The rules.  Of a request's 2 num_beams best candidates, taken in their order: one that ends with a stop token becomes a finished
-hypothesis if it is among the first num_beams, any other becomes a beam until there are num_beams.  A hypothesis of n new tokens scores
+The rules.  A request's candidates are taken in their order: one that ends with a stop token becomes a finished
+hypothesis if it is among the first num_beams, any other becomes a beam until there are num_beams.  (With m stop tokens, num_beams
+of the best (1 + m) num_beams candidates go on, so that many are asked for.)  A hypothesis of n new tokens scores
 (sum of its tokens' log-probabilities) / n ** length_penalty.  The best num_beams hypotheses are kept.  A request ends when
 num_beams are finished and no beam can still do better (with ``early_stopping``: when num_beams are finished), or at
 ``max_new_tokens``, where its beams become hypotheses too.
@@ -40,6 +41,23 @@ class BeamRequest:
             raise ValueError("max_new_tokens must be >= 1")
         if not (1 <= self.num_beams <= K.BEAM_MAX_ROWS):
             raise ValueError(f"num_beams must lie in 1..{K.BEAM_MAX_ROWS}, got {self.num_beams}")
+        if self.num_beams + self.stops > K.BEAM_MAX_CANDIDATES:
+            raise ValueError(f"{self.num_beams} beams and {self.stops} stop tokens; {K.BEAM_MAX_CANDIDATES} in all are taken")
+
+    @property
+    def stops(self) -> int:
+        return len(set(self.stop_token_ids))
+
+    def candidates(self, rows: int) -> int:
+        """How many of the best candidates of ``rows`` beams hold all that may be taken: each beam has at most ``stops`` that end."""
+        return max(2 * self.num_beams, self.num_beams + rows * self.stops)
+
+    def cuts(self, rows: int) -> List[int]:
+        """``rows`` beams in parts whose candidates one selection can give (one part but for many beams with several stop tokens)."""
+        part = rows
+        if self.candidates(rows) > K.BEAM_MAX_CANDIDATES:
+            part = (K.BEAM_MAX_CANDIDATES - self.num_beams) // self.stops
+        return [min(part, rows - at) for at in range(0, rows, part)]
 
 
 @dataclass
@@ -189,18 +207,23 @@ class BeamLoop:
 
     def _step(self, live: List[_Live], first: bool, results: List[BeamResult]) -> List[_Live]:
         beams = [b for l in live for b in l.beams]
-        start = [0]
+        start, first_part = [0], []
         for l in live:
-            start.append(start[-1] + len(l.beams))
+            first_part.append(len(start) - 1)
+            for n in l.request.cuts(len(l.beams)):
+                start.append(start[-1] + n)
+        first_part.append(len(start) - 1)
         feed = [list(l.request.prompt) for l in live] if first else [[b.token] for b in beams]
-        k = max(2 * l.request.num_beams for l in live)
+        k = min(K.BEAM_MAX_CANDIDATES, max(l.request.candidates(len(l.beams)) for l in live))
         scores, rows, tokens = self.backend.select([b.slot for b in beams], feed, [b.score for b in beams], start, k)
         still, moves = [], []
-        for l, sc, rw, tk in zip(live, scores, rows, tokens):
-            found = [j for j in range(2 * l.request.num_beams) if rw[j] >= 0]
+        for l, lo, hi in zip(live, first_part, first_part[1:]):
+            found = [c for part in range(lo, hi) for c in zip(scores[part], rows[part], tokens[part]) if c[1] >= 0]
             if not found:
                 raise RuntimeError(f"request {l.request.request_id}: no continuation has a finite log-probability")
-            l.take([sc[j] for j in found], [beams[rw[j]] for j in found], [tk[j] for j in found])
+            if hi - lo > 1:
+                found.sort(key=lambda c: -c[0])                  # stable: the lower rows first where scores tie
+            l.take([c[0] for c in found], [beams[c[1]] for c in found], [c[2] for c in found])
             if l.over():
                 l.beams = []
                 results[l.index].hypotheses = l.finished

@@ -368,3 +368,60 @@ def test_tokens_by_adapter():
     order, start, ids = got[:12], got[12:17], got[17:]
     assert sorted(order) == list(range(12)) and order[:6] == [3, 0, 1, 4, 5, 6]
     assert start == [0, 1, 6, 6, 6] and ids == [0, 3, -1, -1]
+
+
+# ------------------------------------------------------------------------------------------------------ several stop tokens
+class Ending(Table):
+    """A language that likes to end: tokens 0, 1, ... of ``ends`` have the largest log-probabilities."""
+
+    def __init__(self, ends, **kw):
+        super().__init__(**kw)
+        self.ends, self.live = ends, []
+
+    def logp(self, text, adapter=-1):
+        lp = super().logp(text, adapter)
+        return torch.log_softmax(lp + 3.0 * (torch.arange(self.V) < self.ends), 0)
+
+    def select(self, slots, tokens, scores, start, k):
+        self.live.append(len(slots))
+        assert all(hi - lo <= 64 for lo, hi in zip(start[:-1], start[1:])) and k <= 128
+        return super().select(slots, tokens, scores, start, k)
+
+
+def by_hand_uncut(lang, prompt, n, beams, stop):
+    """The search over all candidates of every step."""
+    live, done, counts = [(0.0, [])], [], []
+    for step in range(1, n + 1):
+        c = sorted(((s + float(lp), i, v, t) for i, (s, t) in enumerate(live) for v, lp in enumerate(lang.logp(prompt + t))),
+                   key=lambda x: (-x[0], x[1], x[2]))
+        live = []
+        for rank, (s, _, v, t) in enumerate(c):
+            if v in stop:
+                if rank < beams:
+                    done.append((s / step, t + [v], "stop"))
+            elif len(live) < beams:
+                live.append((s, t + [v]))
+        counts.append(len(live))
+        done = sorted(done, key=lambda h: -h[0])[:beams]
+        if step == n:
+            done = sorted(done + [(s / n, t, "length") for s, t in live], key=lambda h: -h[0])[:beams]
+        elif len(done) == beams and max(s for s, _ in live) / n <= done[-1][0]:
+            break
+    return done, counts
+
+
+@pytest.mark.parametrize("beams,n,V,ends", [(1, 6, 7, 2), (4, 6, 9, 3), (3, 5, 12, 6), (8, 4, 20, 7), (64, 3, 14, 3), (40, 3, 30, 5), (63, 3, 70, 65)])
+def test_beams_go_on_whatever_the_number_of_stop_tokens(beams, n, V, ends):
+    lang = Ending(ends, V=V, slots=beams)
+    stop = tuple(range(ends)) * 2                # named twice: still so many
+    (r,) = BeamLoop(lang).run([BeamRequest([1], n, beams, stop_token_ids=stop)])
+    want, counts = by_hand_uncut(Ending(ends, V=V), [1], n, beams, stop)
+    assert [h.tokens for h in r.hypotheses] == [t for _, t, _ in want]
+    assert [h.finish_reason for h in r.hypotheses] == [why for _, _, why in want]
+    assert lang.live == [1] + counts[:len(lang.live) - 1] and counts[-1] == min(beams, counts[-2] * (V - ends))
+
+
+def test_more_stop_tokens_than_a_selection_has_room_for_are_refused():
+    BeamRequest([1], 2, 64, stop_token_ids=tuple(range(64)))
+    with pytest.raises(ValueError, match="64 beams and 65 stop tokens"):
+        BeamRequest([1], 2, 64, stop_token_ids=tuple(range(65)))

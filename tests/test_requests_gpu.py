@@ -20,7 +20,7 @@ import revelix_helpers
 from flashdecode_cuda_b200.weights import write_adapter
 from helpers import TINY, TOL, prompts_for, raw_config, rel_err, weights_of, write_folder
 from plain import qwen2_plain as P
-from test_beam import by_hand
+from test_beam import by_hand, by_hand_uncut
 
 pytestmark = pytest.mark.gpu
 ROOT = Path(__file__).resolve().parent.parent
@@ -91,6 +91,21 @@ def test_beam_search_equals_the_search_by_hand(folders, name, beams, n, penalty)
         assert not eng.cache.active_slots()
         eng.cache.check_invariants()
         assert eng.cache.blocks_in_use() == [0] * len(eng.cache.groups)
+
+
+def test_many_beams_with_several_stop_tokens(folders):
+    """More candidates than one selection gives: a request's rows are selected from in parts."""
+    eng = fd.load(folders["B"], device="cuda", dtype="float32")
+    raw = raw_config(folders["B"])
+    lang = Language(raw, {-1: weights_of(folders["B"])})
+    prompt = prompts_for(raw["vocab_size"], [7], seed=12)[0]
+    stop = [int(t) for t in lang.logp(prompt).topk(6).indices]
+    (got,) = eng.beam_search([prompt], 3, num_beams=30, num_return=30, stop_token_ids=stop)
+    want, counts = by_hand_uncut(lang, prompt, 3, 30, stop)
+    assert counts == [30] * len(counts)
+    assert [h.tokens for h in got.hypotheses] == [t for _, t, _ in want]
+    assert all(abs(h.score - s) < 1e-4 for h, (s, _, _) in zip(got.hypotheses, want))
+    eng.model.check_status()
 
 
 def test_one_beam_is_greedy_and_requests_may_differ(folders):
