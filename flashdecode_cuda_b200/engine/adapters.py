@@ -13,6 +13,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from .. import kernels as K
 from ..parts.lowrank import LowRank
 from ..weights.adapters import Adapter
 
@@ -25,6 +26,8 @@ class Adapters:
             raise RuntimeError("the model has no weights yet: adapters come after bind()")
         if capacity < 1 or rank < 1:
             raise ValueError("capacity and rank must be >= 1")
+        if rank > K.LORA_MAX_RANK:
+            raise ValueError(f"adapters of ranks up to {K.LORA_MAX_RANK} are taken, not {rank}")
         self.capacity, self.rank = capacity, rank
         self.made = next(_made)                      # a captured step belongs to the memory of one of these
         self.names: List[Optional[str]] = [None] * capacity

@@ -129,7 +129,8 @@ class Engine(Backend, BeamBackend):
     # -- adapters -------------------------------------------------------------
     def enable_adapters(self, max_adapters: int = 8, max_rank: int = 16) -> Adapters:
         """Room for low-rank adapters beside the model's products, allocated now (at most once).  ``add_adapter`` does this with
-        these sizes, or the first adapter's rank if that is larger, where it has not been done."""
+        these sizes, or the first adapter's rank if that is larger, where it has not been done.  Ranks up to 256, and where
+        projections are one packed product up to 512 in all of them: 168 for q, k and v, 256 for gate and up."""
         if self.model.adapters is not None:
             raise RuntimeError("the model has room for adapters already")
         return Adapters(self.model, max_adapters, max_rank)

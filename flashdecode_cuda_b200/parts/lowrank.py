@@ -13,6 +13,11 @@ from .base import Runtime
 RANK_UNIT = 8       # ranks are stored in multiples of this (16-byte pieces of bfloat16), zeros behind an adapter's own
 
 
+def largest_rank(slices: int) -> int:
+    """The largest rank that a product of so many packed projections has room for."""
+    return min(K.LORA_MAX_RANK, K.LORA_MAX_PACKED // slices) // RANK_UNIT * RANK_UNIT
+
+
 @dataclass
 class AdaptedProduct:
     """A product of a part that takes adapters: ``modules`` are the checkpoint's names of the projections that its matrix packs and
@@ -34,11 +39,14 @@ class TokenAdapters:
 
 
 class LowRank:
-    """The adapters of one product: A [E, slices * R, inputs], B [E, outputs, R]."""
+    """The adapters of one product: A [E, slices * R, inputs], B [E, outputs, R].  R is ``rank``, or what the kernel takes of so many
+    packed projections where that is less."""
 
     def __init__(self, product: AdaptedProduct, capacity: int, rank: int, rt: Runtime):
-        self.product, self.rank, self.rt = product, -(-rank // RANK_UNIT) * RANK_UNIT, rt
         self.slices = len(product.modules)
+        if self.slices > K.LORA_MAX_SLICES:
+            raise ValueError(f"{product.modules[0]}: adapters take up to {K.LORA_MAX_SLICES} packed projections, not {self.slices}")
+        self.product, self.rank, self.rt = product, min(-(-rank // RANK_UNIT) * RANK_UNIT, largest_rank(self.slices)), rt
         N = sum(product.rows)
         which = torch.repeat_interleave(torch.arange(self.slices), torch.tensor(list(product.rows)))
         self.order = torch.arange(N) if product.order is None else product.order.cpu()

@@ -1,0 +1,57 @@
+"""Low-rank adapters without a GPU: the room for them, what is refused before anything is changed."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from flashdecode_cuda_b200 import kernels as K
+from flashdecode_cuda_b200.engine.adapters import Adapters
+from flashdecode_cuda_b200.parts.lowrank import AdaptedProduct, LowRank, largest_rank
+
+RT = SimpleNamespace(device=torch.device("cpu"), dtype=torch.float32, status=None)
+
+
+class Part:
+    lora = None
+
+    def adapted_products(self):
+        return [AdaptedProduct("qkv", ["q_proj", "k_proj", "v_proj"], [32, 16, 16], 24), AdaptedProduct("o", ["o_proj"], [24], 32),
+                AdaptedProduct("gate_up", ["gate_proj", "up_proj"], [40, 40], 24)]
+
+
+def model():
+    parts = [Part(), Part()]
+    return SimpleNamespace(bound=True, rt=RT, all_parts=lambda: parts[:1], adapters=None, parts=parts)
+
+
+def pair(n, k, rank):
+    g = torch.Generator().manual_seed(n + rank)
+    return torch.randn(rank, k, generator=g), torch.randn(n, rank, generator=g)
+
+
+def test_room_is_what_the_kernel_takes():
+    for slices, most in ((1, 256), (2, 256), (3, 168), (4, 128)):
+        assert largest_rank(slices) == most
+        product = AdaptedProduct("p", [f"m{i}" for i in range(slices)], [8] * slices, 16)
+        for rank in (1, 8, most - 7, most, most + 1, 256):
+            low = LowRank(product, 2, rank, RT)
+            assert low.rank == min(-(-rank // 8) * 8, most) and low.rank <= K.LORA_MAX_RANK and low.rank * slices <= K.LORA_MAX_PACKED
+            assert low.a.shape == (2, slices * low.rank, 16) and low.b.shape == (2, 8 * slices, low.rank)
+    with pytest.raises(ValueError, match="up to 4 packed"):
+        LowRank(AdaptedProduct("p", list("abcde"), [8] * 5, 16), 2, 8, RT)
+
+
+def test_a_rank_that_a_product_cannot_take_is_refused_when_the_adapter_is_added():
+    m = model()
+    ad = Adapters(m, 2, 256)
+    assert {k: low.rank for k, low in ad.products.items()} == {"q_proj": 168, "k_proj": 168, "v_proj": 168, "o_proj": 256, "gate_proj": 256, "up_proj": 256}
+    assert ad.put("wide", {"o_proj": pair(24, 32, 256), "q_proj": pair(32, 24, 168)}, 1.0) == 0
+    kept = [(low.a.clone(), low.b.clone(), low.ranks.clone()) for low in ad.products.values()]
+    with pytest.raises(ValueError, match="k_proj: an adapter of rank 169; there is room for 168"):
+        ad.put("wider", {"o_proj": pair(24, 32, 2), "k_proj": pair(16, 24, 169)}, 1.0)
+    assert ad.names == ["wide", None]
+    assert all(torch.equal(x, y) for low, k in zip(ad.products.values(), kept) for x, y in zip((low.a, low.b, low.ranks), k))
+    assert ad.put("small", {"k_proj": pair(16, 24, 4)}, 1.0) == 1
+    with pytest.raises(ValueError, match="up to 256"):
+        Adapters(model(), 2, 257)

@@ -179,6 +179,31 @@ def test_adapters_equal_merged_weights(folders, name, dtype):
             assert rel_err(r[j], want[len(p) - 1 + i]) < TOL[dtype], (j, i)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_largest_ranks(folders, dtype):
+    """Ranks of 256, and of 168 where three projections are one product, beside an adapter of a small rank."""
+    folder = folders["B"]
+    raw = raw_config(folder)
+    eng = fd.load(folder, device="cuda", dtype=dtype)
+    wide = {m: ab for rank, part in ((168, "self_attn"), (256, "mlp"), (256, "o_proj"))
+            for m, ab in adapter_for(folder, rank, rank, lambda m: part in m).items()}
+    small = adapter_for(folder, 3, 4)
+    eng.add_adapter("wide", as_tensors(wide), scale=0.5)
+    eng.add_adapter("small", as_tensors(small), scale=0.5)
+    weights = [merged(folder, wide, 0.5), merged(folder, small, 0.5)]
+    prompts = prompts_for(raw["vocab_size"], [20, 9], seed=15)
+    cache = eng.model.new_cache(max_tokens=64 * 4)
+    slots = [cache.admit(0), cache.admit(1)]
+    first = eng.model.step(cache, slots, prompts, "last").double().cpu()
+    second = eng.model.step(cache, slots, [[5], [6]], "last").double().cpu()
+    eng.model.check_status()
+    for j, w in enumerate(weights):
+        want = P.logits(raw, w, prompts[j] + [5 + j])
+        assert rel_err(first[j], want[len(prompts[j]) - 1]) < TOL[dtype] and rel_err(second[j], want[len(prompts[j])]) < TOL[dtype]
+    with pytest.raises(ValueError, match="q_proj: an adapter of rank 176"):
+        eng.add_adapter("wider", as_tensors(adapter_for(folder, 1, 176, lambda m: "q_proj" in m)), scale=1.0)
+
+
 def test_adapters_in_generation_and_with_beams(folders):
     folder = folders["B"]
     raw = raw_config(folder)
