@@ -146,9 +146,15 @@ class Engine(Backend, BeamBackend):
         else:
             pairs, of_file = A.read_adapter(source)
             scale = of_file if scale is None else scale
+        made = None
         if self.model.adapters is None:
-            self.enable_adapters(max_rank=max(16, max(a.shape[0] for a, _ in pairs.values())))
-        return self.model.adapters.put(name, pairs, float(scale))
+            made = self.enable_adapters(max_rank=max(16, max(a.shape[0] for a, _ in pairs.values())))
+        try:
+            return self.model.adapters.put(name, pairs, float(scale))
+        except Exception:
+            if made is not None:                     # room of a refused adapter's size is nobody's wish
+                made.give_back()
+            raise
 
     def remove_adapter(self, name: str) -> None:
         if self.model.adapters is None:

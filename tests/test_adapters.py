@@ -55,3 +55,31 @@ def test_a_rank_that_a_product_cannot_take_is_refused_when_the_adapter_is_added(
     assert ad.put("small", {"k_proj": pair(16, 24, 4)}, 1.0) == 1
     with pytest.raises(ValueError, match="up to 256"):
         Adapters(model(), 2, 257)
+
+
+def engine(m):
+    from flashdecode_cuda_b200.engine.api import Engine
+    eng = object.__new__(Engine)
+    eng.model, eng.cache, eng._own_cache = m, None, None
+    return eng
+
+
+def named(pairs):
+    return {f"{m}.lora_{h}.weight": t for m, ab in pairs.items() for h, t in zip("AB", ab)}
+
+
+def test_a_refused_first_adapter_leaves_no_room_behind():
+    """Room is allocated once; that of an adapter that was not taken would be too small for the next one."""
+    m = model()
+    eng = engine(m)
+    for bad in ({"lm_head": pair(9, 24, 4)}, {"q_proj": pair(31, 24, 4)}, {"q_proj": pair(32, 24, 200), "o_proj": pair(24, 32, 2)}):
+        with pytest.raises(ValueError):
+            eng.add_adapter("x", named(bad), 1.0)
+        assert m.adapters is None and all(p.lora is None for p in m.parts)
+    with pytest.raises(ValueError, match="needs a name"):
+        eng.add_adapter("", named({"q_proj": pair(32, 24, 4)}), 1.0)
+    assert m.adapters is None
+    assert eng.add_adapter("x", named({"o_proj": pair(24, 32, 40)}), 1.0) == 0 and m.adapters.rank == 40
+    with pytest.raises(ValueError, match="takes no adapter"):
+        eng.add_adapter("y", named({"lm_head": pair(9, 24, 4)}), 1.0)
+    assert m.adapters.names[0] == "x" and m.parts[0].lora is not None       # room that is used stays
