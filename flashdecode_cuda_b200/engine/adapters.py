@@ -44,14 +44,14 @@ class Adapters:
             raise ValueError("no part of this model takes low-rank adapters")
         for part, mine in built:
             part.lora = mine
-        self._model, self._parts = model, [part for part, _ in built]
         model.adapters = self
 
-    def give_back(self) -> None:
+    @staticmethod
+    def give_back(model) -> None:
         """The model has no adapters and no room for any again."""
-        for part in self._parts:
+        for part in model.all_parts():
             part.lora = None
-        self._model.adapters = None
+        model.adapters = None
 
     def index(self, name: Optional[str]) -> int:
         """The number under which sequences use the adapter (-1 for None)."""

@@ -146,14 +146,14 @@ class Engine(Backend, BeamBackend):
         else:
             pairs, of_file = A.read_adapter(source)
             scale = of_file if scale is None else scale
-        made = None
-        if self.model.adapters is None:
-            made = self.enable_adapters(max_rank=max(16, max(a.shape[0] for a, _ in pairs.values())))
+        first = self.model.adapters is None
+        if first:
+            self.enable_adapters(max_rank=max(16, max(a.shape[0] for a, _ in pairs.values())))
         try:
             return self.model.adapters.put(name, pairs, float(scale))
         except Exception:
-            if made is not None:                     # room of a refused adapter's size is nobody's wish
-                made.give_back()
+            if first:                                # room of a refused adapter's size is nobody's wish
+                Adapters.give_back(self.model)
             raise
 
     def remove_adapter(self, name: str) -> None:

@@ -83,3 +83,21 @@ def test_a_refused_first_adapter_leaves_no_room_behind():
     with pytest.raises(ValueError, match="takes no adapter"):
         eng.add_adapter("y", named({"lm_head": pair(9, 24, 4)}), 1.0)
     assert m.adapters.names[0] == "x" and m.parts[0].lora is not None       # room that is used stays
+
+
+def test_a_dropped_model_goes_at_once():
+    """Adapters do not keep their model, nor it itself through them."""
+    import gc
+    import weakref
+
+    class Model(SimpleNamespace):
+        pass
+    m = Model(**vars(model()))
+    Adapters(m, 2, 8)
+    seen = weakref.ref(m), weakref.ref(m.adapters)
+    gc.disable()
+    try:
+        del m
+        assert seen[0]() is None and seen[1]() is None
+    finally:
+        gc.enable()
