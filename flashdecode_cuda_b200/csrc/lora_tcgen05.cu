@@ -12,6 +12,9 @@
 // One warp asks for copies, one thread issues MMAs, eight warps do the rest.  out takes y's place in shared memory, so that it leaves in
 // whole lines although a thread's share of D2 is a row.
 //
+// A wait that runs out before step 2 stops the whole cluster: its sums lack a part, and nothing is stored.  One in step 3 stops its own
+// CTA, whose tiles from there on stay as they were.  Copies and MMAs in flight end before their memory is used again or given up.
+//
 // Measured: four prompts of 1,900 to 2,048 tokens, 13824 x 5120, rank 64 (390 MB, floor 59.7 us): 93 us, 4.2 TB/s - finding the tile 3, step 1 47
 // (an SM takes 57 GB/s, a third of it A, which every tile reads anew out of L2), step 2 5, step 3 32 (5.1 TB/s of y and out).  The two
 // streams follow one another, the exchange stands between them, and 65 tiles in clusters of 2 leave 18 SMs idle.  Tensor pipe 11 %.
@@ -83,6 +86,14 @@ __device__ __forceinline__ void lt_ld8(uint32_t taddr, uint32_t* v) {
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
 }
 
+// A barrier of the epilogue's warps: whether all of them are well.
+__device__ __forceinline__ bool lt_all_epi(bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((uint32_t)ok), "n"(LT_EPI * 32) : "memory");
+    return all != 0;
+}
+
 // x and y in boxes of 128 rows, of 16, and of one (for gathers).
 struct LoraMaps {
     CUtensorMap x[3], y[3], a, b;
@@ -127,7 +138,7 @@ struct LoraRows {
 
 __global__ void __launch_bounds__(LT_THREADS, 1)
 lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const int chunks, const int stages, const int out_stages,
-                 const unsigned long long wait_ns) {
+                 const unsigned long long wait_ns, const int skip_last) {
     extern __shared__ unsigned char lt_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)lt_smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) unsigned long long full[LT_RING], empty[LT_RING], out_full[LT_OUT_RING], out_empty[LT_OUT_RING], acc_full[2],
@@ -194,6 +205,7 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
 
     // ---- 1. D1 = x A^T over this CTA's share of K ----
     const LoraRows rows(tok, tile.count);
+    int asked = 0;                                               // blocks, then tiles, that warp 0 has asked for
     if (warp == 0) {
         for (int it = 0; it < nb; ++it) {
             const int s = it % stages, k = (b0 + it) * 64;
@@ -202,7 +214,10 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
             if (lane == 0) mbar_expect_tx(bar, stage_bytes);
             __syncwarp();
             if (rows.all && lane == 0) tma_load_2d(at, maps.x, bar, k, rows.first);
-            if (lane < p.S) tma_load_2d(at + LT_TILE + lane * r16 * 128, &maps.a, bar, k, (e * p.S + lane) * p.R);
+            // (tests: a cluster's first CTA leaves out one copy of its last block)
+            if (lane < p.S && !(skip_last == 1 && rank == 0 && it == nb - 1 && lane == 0))
+                tma_load_2d(at + LT_TILE + lane * r16 * 128, &maps.a, bar, k, (e * p.S + lane) * p.R);
+            ++asked;
         }
     } else if (warp == 1 && lane == 0) {
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(W >> 3) << 17) | ((uint32_t)(LT_ROWS >> 4) << 24);
@@ -237,9 +252,21 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
     // ---- 2. the cluster's sums ----
     const int quarter = warp & 3, half = (warp - 2) >> 2, et = tid - 64;         // of the epilogue warps: the lanes of tensor memory, the columns
     float* part = reinterpret_cast<float*>(smem + 2 * hbytes);   // [128][W + 4]
+    volatile int* const gave_up = &abort_flag;
+    if (warp >= 2) mbar_wait(s_addr(&d1_full), 0, &abort_flag, p.status, wait_ns);
+    __syncthreads();
+    // Every MMA of step 1 has ended then, and if no wait ran out every copy: the ring's memory is free.  Else the copies are waited for:
+    // those that warp 0 has asked for, and, where others ask too, what they may have asked for beyond (which nobody completes).
+    if (*gave_up) {
+        if (warp == 0) {
+            int here = 0;
+            for (int it = max(0, asked - stages); it < min(nb, asked + (rows.all ? 0 : 1)); ++it)
+                mbar_wait(s_addr(&full[it % stages]), (it / stages) & 1, &here, nullptr, wait_ns);
+        }
+        __syncthreads();
+    }
     if (warp >= 2) {
-        // (every copy and MMA of step 1 has ended then: the ring's memory is free)
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(s_addr(&d1_full), 0, &abort_flag, p.status, wait_ns)) && nb > 0;
+        const bool ok = !*gave_up && nb > 0;
         tc_fence_after();
         const int row = quarter * 32 + lane;
         for (int c0 = half * 16; c0 < W; c0 += 32) {
@@ -259,6 +286,7 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
     }
     __syncwarp();
     cluster.sync();
+    const int lacks = lane < C ? *cluster.map_shared_rank(&abort_flag, lane) : 0;          // (nobody waits with it until the next barrier)
     {
         const int share = LT_ROWS / C, per_row = W / 8;
         for (int i = tid; i < share * per_row; i += LT_THREADS) {
@@ -283,15 +311,17 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
         }
     }
     asm volatile("fence.proxy.async;" ::: "memory");             // written by threads, read by the MMAs of any CTA; and part's memory takes copies
-    __syncwarp();
+    const int end = __any_sync(0xffffffffu, lacks) ? 0 : tiles;  // a sum that lacks a part: no tile is computed
     cluster.sync();
     asm volatile("fence.proxy.async;" ::: "memory");
 
     // ---- 3. out = y + scale h B^T for this CTA's tiles of 128 columns ----
     const uint32_t ring = base + 2 * hbytes;                     // stages: y, then B
+    asked = 0;
+    int issued = 0;                                              // tiles whose MMAs warp 1 has issued
     if (warp == 0) {
         int i = 0;
-        for (int t = rank; t < tiles; t += C, ++i) {
+        for (int t = rank; t < end; t += C, ++i) {
             const int s = i % out_stages, n0 = t * LT_COLS;
             if (i >= out_stages && !__all_sync(0xffffffffu, mbar_wait(s_addr(&out_empty[s]), (i / out_stages - 1) & 1, &abort_flag, p.status, wait_ns))) break;
             const uint32_t bar = s_addr(&out_full[s]), at = ring + s * out_stage_bytes;
@@ -300,19 +330,16 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
             __syncwarp();
             rows.ask(at, maps.y, bar, n0);
             if (both) rows.ask(at + LT_TILE, maps.y, bar, n0 + 64);
-            if (lane < chunks) tma_load_2d(at + LT_Y_BYTES + lane * LT_TILE, &maps.b, bar, lane * 64, e * p.N + n0);
-        }
-        // copies that nobody waited for (after a wait that gave up) end before their memory is given up
-        if (abort_flag) {
-            int here = 0;
-            for (int j = max(0, i - out_stages); j < i; ++j) mbar_wait(s_addr(&out_full[j % out_stages]), (j / out_stages) & 1, &here, nullptr, wait_ns);
-            for (int it = max(0, nb - stages); it < nb; ++it) mbar_wait(s_addr(&full[it % stages]), (it / stages) & 1, &here, nullptr, wait_ns);
+            // (tests: each CTA leaves out one copy of its last tile)
+            if (lane < chunks && !(skip_last == 2 && t + C >= end && lane == 0))
+                tma_load_2d(at + LT_Y_BYTES + lane * LT_TILE, &maps.b, bar, lane * 64, e * p.N + n0);
+            ++asked;
         }
     } else if (warp == 1) {
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LT_COLS >> 3) << 17) | ((uint32_t)(LT_ROWS >> 4) << 24);
         const int steps = (r + 15) / 16;                         // as far as the adapter's rank reaches
         int i = 0;
-        for (int t = rank; t < tiles; t += C, ++i) {
+        for (int t = rank; t < end; t += C, ++i) {
             const int s = i % out_stages, acc = i % accs, n = t * LT_COLS + (lane & 15) * 8;
             // the slices that have columns in this tile
             const unsigned present = p.col_slice == nullptr ? 1u
@@ -333,12 +360,13 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
                 }
                 tc_commit(s_addr(&acc_full[acc]));
             }
+            ++issued;
             __syncwarp();
         }
     } else {
         const float scale = p.scale[e];
         int i = 0;
-        for (int t = rank; t < tiles; t += C, ++i) {
+        for (int t = rank; t < end; t += C, ++i) {
             const int s = i % out_stages, acc = i % accs, n0 = t * LT_COLS;
             // lane j < 8: the slice of this warp's group j of 8 columns
             const int n = n0 + half * 64 + (lane & 7) * 8;
@@ -377,10 +405,10 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_addr(&acc_empty[acc]));
-            asm volatile("bar.sync 1, %0;" ::"n"(LT_EPI * 32) : "memory");
+            if (!lt_all_epi(ok)) break;                          // a warp stores what all of them have left: all of the tile, or nothing from here on
             // rows in whole lines: 16 lanes a row
             const int chunk = et & 15, col = n0 + chunk * 8;
-            if (ok && col < p.N) {
+            if (col < p.N) {
                 const unsigned char* from = stage + (chunk >> 3) * LT_TILE;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -397,6 +425,17 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (*gave_up) {                                              // copies and MMAs that nobody waited for
+        int here = 0;
+        if (warp == 0)
+            for (int i = max(0, asked - out_stages); i < asked; ++i)
+                mbar_wait(s_addr(&out_full[i % out_stages]), (i / out_stages) & 1, &here, nullptr, wait_ns);
+        if (warp == 1) {
+            mbar_wait(s_addr(&d1_full), 0, &here, nullptr, wait_ns);
+            for (int i = max(0, issued - accs); i < issued; ++i) mbar_wait(s_addr(&acc_full[i % accs]), (i / accs) & 1, &here, nullptr, wait_ns);
+        }
+        __syncwarp();
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -437,7 +476,7 @@ int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream) {
         once.done();
     }
     return launch("lora_add", lora_tile_kernel, dim3((unsigned)(tiles * C)), dim3(LT_THREADS), f.smem, stream, dim3(C, 1, 1), maps, p, f.chunks,
-                  f.stages, f.out_stages, g_tc_wait_ns);
+                  f.stages, f.out_stages, g_tc_wait_ns, g_tc_skip_last);
 }
 
 }  // namespace fd

@@ -697,7 +697,8 @@ def tc_test_hook(wait_ns: int = 0, skip_last: int = 0) -> None:
     """Tests only.  The limit of every bounded wait of the TMA + tcgen05 kernels (0: the default of
     0.2 s) and whether their producers leave out their very last copy, so that a wait runs out and the
     kernel reports ``STATUS_WAIT_TIMEOUT`` and returns.  In a one-kernel decode step one CTA keeps words of the last layer
-    to itself: 1 its normed stream, 2 its queries, 3 its attention, 4 its partial sums of the down projection."""
+    to itself: 1 its normed stream, 2 its queries, 3 its attention, 4 its partial sums of the down projection.  In ``lora_add``'s tiles of
+    128 tokens the copy left out is 1 one of a cluster's last columns of x and a, 2 one of each CTA's last columns of b."""
     lib().fd_tc_test_hook(int(wait_ns), int(skip_last))
 
 

@@ -395,3 +395,29 @@ def test_a_float32_token_has_the_same_bits_in_any_step(Kd, N, R, S):
     for some in ([0], [5, 1299, 700], list(range(3, 560)), list(range(0, 1300, 2))):
         part = dict(d, x=d["x"][some], y=d["y"][some])
         assert torch.equal(run(part, cols, S, [token[t] for t in some]), want[some])
+
+
+@pytest.mark.parametrize("tokens", ["neighbours", "here and there"])
+@pytest.mark.parametrize("Kd,C", [(64, 1), (192, 2), (520, 8)])
+@pytest.mark.parametrize("kept", [1, 2])
+def test_waits_that_run_out_in_tiles_of_128(kept, Kd, C, tokens):
+    """One copy never leaves.  For the sums over K: its whole cluster stores nothing, whichever of its CTAs waited.  For b: the columns
+    before it are right, those from there on are left as they were.  The status says so, and the next call is right."""
+    T, N, R = 300, 20 * 128, 16
+    d, cols, S = make("bfloat16", T, Kd, N, 2, R)
+    token = [i * 2 // T for i in range(T)] if tokens == "neighbours" else [(i * 5 // 3) % 2 for i in range(T)]
+    K.lora_set_form(2)
+    try:
+        want = run(d, cols, S, token)
+        st = torch.zeros(1, dtype=torch.int32, device=DEV)
+        K.tc_test_hook(wait_ns=1_000_000, skip_last=kept)
+        got = run(d, cols, S, token, status=st)
+        assert int(st.item()) == K.STATUS_WAIT_TIMEOUT
+        done = 0 if kept == 1 else (20 - C) * 128                # of 20 tiles each CTA's last is not computed
+        assert torch.equal(got[:, :done], want[:, :done]) and bool((got[:, done:] == 9.0).all())
+        K.tc_test_hook()
+        st.zero_()
+        assert torch.equal(run(d, cols, S, token, status=st), want) and int(st.item()) == 0
+    finally:
+        K.tc_test_hook()
+        K.lora_set_form(0)
