@@ -20,9 +20,8 @@
 // Why the sums are in 64 bits: which of two candidates of different beams comes first hangs on the difference of two
 // normalisers.  In 32 bits they are off by some 1e-6, and among the candidates of a large batch two that are nearer than
 // that are common (gaps of 1e-2 between neighbours: one pair in ten thousand, and a step of 64 requests has a thousand pairs).  The
-// exponentials themselves are taken in 32 bits, 2^(d log2 e) of differences d = x - max that are exact or off by half a step, with log2 e as
-// the sum of two numbers (one alone is off by 2^-26 of itself, the same way for every entry); what errors of 1e-7 are left have
-// no common sign and average out over the row.  Groups of 16 are added in 32 bits, then in 64.
+// exponentials themselves are taken in 32 bits, of differences d = x - max that are exact or off by half a step (beam_exp); what errors of
+// 1e-7 are left have no common sign and average out over the row.  Groups of 16 are added in 32 bits, then in 64.
 #include <cooperative_groups.h>
 #include <math.h>
 #include <type_traits>
@@ -73,13 +72,15 @@ static BeamPlan beam_plan(int n, int V) {
     return p;
 }
 
-// exp(d) for d <= 0, off by about 2^-22 of itself at most; 0 for -inf.
+// exp(d) for d <= 0; 0 for -inf, NaN for NaN.  2^p of p = d log2 e, times 1 + rest: what the rounding of p leaves out, which alone would make
+// it off by |d| 2^-24.  Over every float: off by 3.3 2^-24 of itself at most down to -33, from there (where it hardly counts in a sum
+// that has a 1) by up to 5.5 at -87, since log2 e and ln 2 are rounded too.
 __device__ __forceinline__ float beam_exp(float d) {
-    constexpr float LOG2E_HI = 1.44269502162933349609375f;       // log2 e rounded down, and what is left of it
-    constexpr float LOG2E_LO = 1.92596299112661746887e-8f;
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(d, LOG2E_LO, d * LOG2E_HI)));
-    return r;
+    asm("max.NaN.f32 %0, %0, 0fC3480000;" : "+f"(d));            // -200: 2^p is 0 from there on, and the rest a number
+    const float p = __fmul_rn(d, 1.44269502162933349609375f), rest = fmaf(p, -0.693147182464599609375f, d);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p));
+    return fmaf(r, rest, r);
 }
 
 // A warp's share of one row: units g, g + stride, ... of those before `end`, BM_BATCH neighbours at a time.  The maxima of their groups

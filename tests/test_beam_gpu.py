@@ -312,3 +312,29 @@ def test_many_rows_of_nearly_the_same_score(form, V, beams, k):
         check(torch.round(2.0 * x) / 2.0, scores, start, k)          # ties within every row
     finally:
         K.beam_select_set_form(0)
+
+
+def test_exponentials_of_far_entries():
+    """Rows of a few zeros and very many entries of one value d, at which the product d log2 e has the largest roundings: what a normaliser
+    is off by is what exp(d) is.  Zeros where every warp begins, so that all of them count from 0.  Bound: exp(d) is off by 4 2^-24 of
+    itself, the sum of 16 equal ones by one rounding (8 of them are exact, 12 not; 16 again), which is another."""
+    V = 1 << 22
+    x = torch.empty(1, V, device=DEV)
+    zeros = (torch.arange(0, V, 2048 * 128)[:, None] + torch.arange(0, 64, 4) * 128).flatten().to(DEV)
+    d = torch.linspace(-8.75, -8.4, 20001)
+    log2e = torch.tensor(math.log2(math.e), dtype=torch.float64)
+    off = (d * log2e.float()).double() - d.double() * log2e
+    order = off.argsort()
+    K.beam_select_set_form(1)
+    try:
+        for v in d[torch.cat([order[:12], order[-12:]])].tolist():
+            x.fill_(v)
+            x[0, zeros] = 0.0
+            tail = (V - len(zeros)) * math.exp(v)
+            lse = math.log(len(zeros) + tail)
+            s = torch.tensor([lse])                              # the best candidate's score is then what both are off by
+            got = select(x, s, [0, 1], 1)
+            share = tail / (len(zeros) + tail)
+            assert abs(float(got[0]) - (float(s) - lse)) <= 5 * 2.0 ** -24 * share + 2.0 ** -40, v
+    finally:
+        K.beam_select_set_form(0)
