@@ -9,6 +9,7 @@ adapter is chosen when its slot is admitted; a step sorts its tokens by adapter 
 from __future__ import annotations
 
 import itertools
+import weakref
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -18,6 +19,16 @@ from ..parts.lowrank import LowRank
 from ..weights.adapters import Adapter
 
 _made = itertools.count(1)
+
+
+class Caches(weakref.WeakSet):
+    """The caches whose sequences a model runs: adapters that they use stay.  A copied model has its own."""
+
+    def __deepcopy__(self, memo):
+        return Caches()
+
+    def use(self, adapter: int) -> bool:
+        return any(cache.adapter(slot) == adapter for cache in self for slot in cache.active_slots())
 
 
 class Adapters:

@@ -157,10 +157,13 @@ class Engine(Backend, BeamBackend):
             raise
 
     def remove_adapter(self, name: str) -> None:
+        """Make room for another adapter.  Refused while a sequence of any cache of the model uses this one."""
         if self.model.adapters is None:
             raise KeyError(f"there is no adapter {name!r}")
         index = self.model.adapters.index(name)
-        if any(c is not None and any(c.adapter(s) == index for s in c.active_slots()) for c in (self.cache, self._own_cache)):
+        if self.cache is not None:
+            self.model.caches.add(self.cache)
+        if self.model.caches.use(index):
             raise RuntimeError(f"adapter {name!r} is in use by a live sequence")
         self.model.adapters.remove(name)
 

@@ -25,6 +25,7 @@ from ..parts.base import KVRequest, LayerCache, Runtime
 from ..parts.lowrank import TokenAdapters
 from ..registry import architecture, part_class
 from ..weights import loader as W
+from .adapters import Caches
 from .blueprint import ModelBlueprint, PartSpec
 from .native import DensePrompts
 
@@ -160,6 +161,7 @@ class Model:
         self.last_meta_host: Optional[np.ndarray] = None        # the index array of the last prepared step
         self.bound = False
         self.adapters = None             # ``engine.adapters.Adapters`` once there are any
+        self.caches = Caches()
         # prompt steps of dense models are launched from native code; None: every step goes through the parts
         self.native: Optional[DensePrompts] = None
 
@@ -316,6 +318,7 @@ class Model:
         cache = PagedCache(groups, states, num_blocks, slots, -(-longest // block_size), block_size,
                            self.dtype, self.device)
         cache.max_len = longest
+        self.caches.add(cache)
         return cache
 
     def _layer_caches(self, cache: PagedCache) -> List[LayerCache]:
@@ -379,6 +382,7 @@ class Model:
             np.asarray(wanted, dtype=np.int32)])
         n_seg = self.adapter_segments(cache, slots, N)
         if n_seg:
+            self.caches.add(cache)       # (one that new_cache did not make)
             host = np.concatenate([host, self.token_adapters(cache, slots, counts, T, n_seg)])
         ws = ws or self.ws
         meta = ws.get("step_meta", (host.size,), torch.int32)

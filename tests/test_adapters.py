@@ -1,12 +1,14 @@
 """Low-rank adapters without a GPU: the room for them, what is refused before anything is changed."""
 
+import copy
 from types import SimpleNamespace
 
 import pytest
 import torch
 
 from flashdecode_cuda_b200 import kernels as K
-from flashdecode_cuda_b200.engine.adapters import Adapters
+from flashdecode_cuda_b200.cache import KVGroupSpec, PagedCache
+from flashdecode_cuda_b200.engine.adapters import Adapters, Caches
 from flashdecode_cuda_b200.parts.lowrank import AdaptedProduct, LowRank, largest_rank
 
 RT = SimpleNamespace(device=torch.device("cpu"), dtype=torch.float32, status=None)
@@ -22,7 +24,7 @@ class Part:
 
 def model():
     parts = [Part(), Part()]
-    return SimpleNamespace(bound=True, rt=RT, all_parts=lambda: parts[:1], adapters=None, parts=parts)
+    return SimpleNamespace(bound=True, rt=RT, all_parts=lambda: parts[:1], adapters=None, parts=parts, caches=Caches())
 
 
 def pair(n, k, rank):
@@ -101,3 +103,29 @@ def test_a_dropped_model_goes_at_once():
         assert seen[0]() is None and seen[1]() is None
     finally:
         gc.enable()
+
+
+def small_cache():
+    return PagedCache([KVGroupSpec(1, 1, 8, None)], [], 8, 4, 2, 4, torch.float32, "cpu")
+
+
+def test_an_adapter_of_a_live_sequence_stays_whatever_the_cache():
+    m = model()
+    eng = engine(m)
+    for name in ("x", "y"):
+        eng.add_adapter(name, named({"q_proj": pair(32, 24, 4)}), 1.0)
+    mine, other = small_cache(), small_cache()
+    m.caches.add(mine)                           # as a model does with the caches that it makes or runs
+    slot = mine.admit(1)
+    with pytest.raises(RuntimeError, match="in use"):
+        eng.remove_adapter("y")
+    mine.release(slot)
+    other.admit(1)
+    eng.cache = other                            # the engine's own
+    with pytest.raises(RuntimeError, match="in use"):
+        eng.remove_adapter("y")
+    assert not m.caches.use(0) and copy.deepcopy(m.caches) is not m.caches and len(copy.deepcopy(m.caches)) == 0
+    eng.cache = None
+    del other                                    # a cache that is gone holds nothing
+    eng.remove_adapter("y")
+    assert m.adapters.names[:2] == ["x", None]

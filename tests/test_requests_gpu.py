@@ -17,6 +17,7 @@ import gulozen_helpers
 import lonasun_helpers
 import nizazen_helpers
 import revelix_helpers
+from flashdecode_cuda_b200.cache import PagedCache
 from flashdecode_cuda_b200.weights import write_adapter
 from helpers import TINY, TOL, prompts_for, raw_config, rel_err, weights_of, write_folder
 from plain import qwen2_plain as P
@@ -302,6 +303,25 @@ def test_adapter_refusals(folders, tmp_path):
     lonasun = fd.load(lonasun_helpers.write_folder(tmp_path, "Z"), device="cuda", dtype="float32")
     with pytest.raises(ValueError, match="no part"):
         lonasun.enable_adapters()
+
+
+def test_adapters_of_sequences_in_any_cache_stay(folders):
+    eng = fd.load(folders["B"], device="cuda", dtype="float32")
+    for i in range(2):
+        eng.add_adapter(str(i), as_tensors(adapter_for(folders["B"], i, 4)), scale=1.0)
+    mine = eng.model.new_cache(max_tokens=128)
+    first = eng.model.new_cache(max_tokens=128)
+    by_hand_made = PagedCache(*eng.model._layout[:2], 8, 2, 4, 16, torch.float32, "cuda")
+    for cache, step in ((mine, False), (by_hand_made, True)):
+        slot = cache.admit(1)
+        if step:
+            eng.model.step(cache, [slot], [[1, 2, 3]])
+        with pytest.raises(RuntimeError, match="in use"):
+            eng.remove_adapter("1")
+        cache.release(slot)
+    slot = first.admit(0)
+    eng.remove_adapter("1")
+    eng.model.check_status()
 
 
 def test_command_line(folders, tmp_path):
