@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import itertools
 import weakref
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -31,6 +31,10 @@ class Caches(weakref.WeakSet):
         return any(cache.adapter(slot) == adapter for cache in self for slot in cache.active_slots())
 
 
+class _Held(list):
+    """(a list that can be referred to weakly)"""
+
+
 class Adapters:
     def __init__(self, model, capacity: int, rank: int):
         if not model.bound:
@@ -42,6 +46,7 @@ class Adapters:
         self.capacity, self.rank = capacity, rank
         self.made = next(_made)                      # a captured step belongs to the memory of one of these
         self.names: List[Optional[str]] = [None] * capacity
+        self._waiting = weakref.WeakValueDictionary()
         self.products: Dict[str, LowRank] = {}       # by module
         built: List[Tuple[object, Dict[str, LowRank]]] = []
         for part in {id(p): p for p in model.all_parts()}.values():
@@ -72,6 +77,16 @@ class Adapters:
             return self.names.index(name)
         except ValueError:
             raise KeyError(f"there is no adapter {name!r}; there are {[n for n in self.names if n]}") from None
+
+    def hold(self, requests: Sequence) -> Sequence:
+        """Requests that are fed bit by bit: the adapters that they name stay until nobody has them any more."""
+        held = _Held(requests)
+        if any(r.adapter >= 0 for r in held):
+            self._waiting[id(held)] = held
+        return held
+
+    def held(self, index: int) -> bool:
+        return any(r.adapter == index for requests in self._waiting.values() for r in requests)
 
     def put(self, name: str, pairs: Adapter, scale: float) -> int:
         """Add an adapter, or replace the one of that name.  Its matrices take effect with the next step."""

@@ -157,7 +157,8 @@ class Engine(Backend, BeamBackend):
             raise
 
     def remove_adapter(self, name: str) -> None:
-        """Make room for another adapter.  Refused while a sequence of any cache of the model uses this one."""
+        """Make room for another adapter.  Refused while a sequence of any cache of the model, or a request of a ``stream`` that has
+        not ended, uses this one."""
         if self.model.adapters is None:
             raise KeyError(f"there is no adapter {name!r}")
         index = self.model.adapters.index(name)
@@ -165,6 +166,8 @@ class Engine(Backend, BeamBackend):
             self.model.caches.add(self.cache)
         if self.model.caches.use(index):
             raise RuntimeError(f"adapter {name!r} is in use by a live sequence")
+        if self.model.adapters.held(index):
+            raise RuntimeError(f"adapter {name!r} is in use by a stream that has not ended")
         self.model.adapters.remove(name)
 
     def _adapter_numbers(self, adapter, n: int) -> List[int]:
@@ -241,6 +244,8 @@ class Engine(Backend, BeamBackend):
         requests = self._requests(input_ids, max_new_tokens, temperature, stop_token_ids, adapter)
         max_batch = self._ensure_cache(requests, cache, max_batch, block_size)
         self.seed = seed
+        if self.model.adapters is not None:
+            requests = self.model.adapters.hold(requests)        # (their adapters' numbers are taken: sequences start later)
         return GenerationLoop(self, max_batch).events(requests)
 
     def beam_search(self, input_ids, max_new_tokens, cache: Optional[PagedCache] = None, *, num_beams: int = 4,

@@ -129,3 +129,30 @@ def test_an_adapter_of_a_live_sequence_stays_whatever_the_cache():
     del other                                    # a cache that is gone holds nothing
     eng.remove_adapter("y")
     assert m.adapters.names[:2] == ["x", None]
+
+
+def test_an_adapter_that_a_stream_waits_for_stays():
+    """A stream's requests have their adapters' numbers before their sequences start."""
+    m = model()
+    eng = engine(m)
+    for name in ("x", "y"):
+        eng.add_adapter(name, named({"q_proj": pair(32, 24, 4)}), 1.0)
+    eng.device = torch.device("cpu")
+    eng.cache = None
+    cache = small_cache()
+    eng.run = lambda slots, tokens, requests, steps: [3] * len(slots)
+    stream = eng.stream([[1], [2], [1]], 2, cache, max_batch=1, adapter=[None, "y", None])
+    for _ in range(2):                           # not begun; then its second request still waits
+        with pytest.raises(RuntimeError, match="stream"):
+            eng.remove_adapter("y")
+        next(stream)
+    eng.remove_adapter("x")
+    next(stream)                                 # the second request's first token
+    with pytest.raises(RuntimeError, match="live sequence"):
+        eng.remove_adapter("y")
+    assert len(list(stream)) == 3
+    eng.remove_adapter("y")
+    eng.add_adapter("y", named({"q_proj": pair(32, 24, 4)}), 1.0)
+    stream = eng.stream([[1], [2]], 2, cache, adapter="y")
+    del stream                                   # never begun
+    eng.remove_adapter("y")
