@@ -61,7 +61,10 @@ static LoraTilePlan lora_tile_plan(const LoraArgs& p) {
     return f;
 }
 
-bool lora_tiles_take(const LoraArgs& p) { return lora_tile_plan(p).stages > 0; }
+// (a copy's row of a or b is a 32-bit number)
+bool lora_tiles_take(const LoraArgs& p) {
+    return (long long)p.E * p.N < (1ll << 31) && (long long)p.E * p.S * p.R < (1ll << 31) && lora_tile_plan(p).stages > 0;
+}
 
 // CTAs of a tile, by the tiles that there should be: T / 128, and a part of one for each segment's last.  One tile too many for a wave costs
 // some 15 to 20 % over clusters of half the size (34 tiles of 3584 x 3584, rank 32: 54 us, 45 in clusters of 2), clusters of half the size
@@ -459,7 +462,6 @@ int lora_tiles(const LoraArgs& p, int sms, cudaStream_t stream) {
     const long long tiles = lora_max_tiles(p, LT_ROWS);
     const int C = lora_tile_cluster(p, sms);
     FD_REQUIRE(tiles * C < (1ll << 31), -2, "lora_add: %d tokens", p.T);
-    FD_REQUIRE((long long)p.E * p.N < (1ll << 31) && (long long)p.E * p.S * p.R < (1ll << 31), -2, "lora_add: %d adapters of %d rows", p.E, p.N);
     LoraMaps maps;
     int rc = lora_map(&maps.a, p.a, (long long)p.E * p.S * p.R, p.K, (p.R + 15) / 16 * 16);
     if (rc == 0) rc = lora_map(&maps.b, p.b, (long long)p.E * p.N, p.R, LT_COLS);

@@ -421,3 +421,30 @@ def test_waits_that_run_out_in_tiles_of_128(kept, Kd, C, tokens):
     finally:
         K.tc_test_hook()
         K.lora_set_form(0)
+
+
+@pytest.mark.parametrize("form", [0, 2])
+@pytest.mark.parametrize("T", [3, 2600])
+def test_more_rows_of_b_than_a_copy_can_name(T, form):
+    """2^31 rows of b (34 GB): steps of any length are taken, by the form that can name them."""
+    E, N, R, Kd = 1 << 17, 1 << 14, 8, 64
+    g = torch.Generator().manual_seed(T)
+    x, y = torch.randn(T, Kd, generator=g).bfloat16().to(DEV), torch.randn(T, N, generator=g).bfloat16().to(DEV)
+    a, b = torch.empty(E, R, Kd, dtype=torch.bfloat16, device=DEV), torch.empty(E, N, R, dtype=torch.bfloat16, device=DEV)
+    for e in (0, E - 1):
+        a[e], b[e] = (torch.randn(R, Kd, generator=g) / 8).bfloat16(), torch.randn(N, R, generator=g).bfloat16()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(y)
+    K.lora_set_form(form)
+    try:
+        K.lora_add(x, a, b, torch.ones(E, device=DEV), torch.full((E,), R, dtype=torch.int32, device=DEV), i32(list(range(T))),
+                   i32([0, T // 2, T]), i32([E - 1, 0]), y, out, status=st)
+    finally:
+        K.lora_set_form(0)
+    assert int(st.item()) == 0
+    for t in (0, T // 2, T - 1):
+        e = E - 1 if t < T // 2 else 0
+        small = dict(x=x[t:t + 1].cpu(), a=a[e:e + 1].cpu(), b=b[e:e + 1].cpu(), y=y[t:t + 1].cpu(), scale=torch.ones(1))
+        want, size, hsize = expected(small, None, 1, [0])
+        assert bool(((out[t:t + 1].cpu().double() - want).abs() <= tolerance("bfloat16", small, want, size, hsize)).all())
