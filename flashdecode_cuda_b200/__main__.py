@@ -32,6 +32,7 @@ def _prompts(args) -> list:
 
 def cmd_generate(args) -> int:
     import flashdecode_cuda_b200 as fd
+    from flashdecode_cuda_b200.engine import NoContinuation
     if args.model:
         engine = fd.load(args.model, device=args.device, dtype=args.dtype)
     else:
@@ -49,15 +50,20 @@ def cmd_generate(args) -> int:
     cache = engine.new_paged_cache(max_batch, longest, args.block_size)
     t0 = time.time()
     if args.beams:
-        found = engine.beam_search(prompts, args.max_new_tokens, cache, num_beams=args.beams, length_penalty=args.length_penalty,
-                                   stop_token_ids=stop, max_batch=max_batch, adapter=adapter)
+        try:
+            found, failed = engine.beam_search(prompts, args.max_new_tokens, cache, num_beams=args.beams, length_penalty=args.length_penalty,
+                                               stop_token_ids=stop, max_batch=max_batch, adapter=adapter), None
+        except NoContinuation as e:
+            found, failed = [r for r in e.results if r.hypotheses], e
         dt = time.time() - t0
         for r in found:
             h = r.hypotheses[0]
             print(json.dumps({"request": r.request_id, "tokens": h.tokens, "finish_reason": h.finish_reason, "score": h.score}))
         n = sum(len(r.tokens) for r in found)
         print(f"{n} tokens in {dt:.3f} s ({n / dt:.1f} tok/s of the best hypotheses, prompts included in the time)", file=sys.stderr)
-        return 0
+        if failed is not None:
+            print(failed, file=sys.stderr)
+        return 0 if failed is None else 1
     results = engine.generate(prompts, args.max_new_tokens, cache, temperature=args.temperature,
                               seed=args.sample_seed, stop_token_ids=stop, max_batch=max_batch, adapter=adapter)
     dt = time.time() - t0

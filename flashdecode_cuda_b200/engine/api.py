@@ -24,7 +24,7 @@ from ..sampling.sampler import Sampler
 from ..weights import adapters as A
 from ..weights import loader as W
 from .adapters import Adapters
-from .beam import BeamBackend, BeamLoop, BeamRequest, BeamResult
+from .beam import BeamBackend, BeamLoop, BeamRequest, BeamResult, NoContinuation
 from .decode import GraphDecoder
 from .generate import Backend, GenerationLoop, Request, Result
 from .model import Model
@@ -255,7 +255,7 @@ class Engine(Backend, BeamBackend):
         """The ``num_return`` best of the hypotheses that beam search over ``num_beams`` beams finds for every prompt
         (``engine.beam`` has its rules), up to ``max_new_tokens`` tokens long.  ``num_beams`` and ``max_new_tokens``: a number, or one
         per prompt.  ``max_batch``: beams that run together (more prompts run as several batches); ``adapter`` as for
-        ``generate``."""
+        ``generate``.  ``NoContinuation``, whose ``results`` are those of the other prompts, where a prompt's logits leave nothing."""
         prompts = self._prompts(input_ids)
         n = len(prompts)
         mx = list(max_new_tokens) if isinstance(max_new_tokens, (list, tuple)) else [max_new_tokens] * n
@@ -270,7 +270,12 @@ class Engine(Backend, BeamBackend):
         if not requests:
             return []
         max_batch = self._ensure_cache(requests, cache, max_batch or max(max(nb), min(sum(nb), 64)), block_size)
-        results = BeamLoop(self, max_batch).run(requests)
+        try:
+            results = BeamLoop(self, max_batch).run(requests)
+        except NoContinuation as e:
+            for r in e.results:
+                del r.hypotheses[num_return:]
+            raise
         for r in results:
             del r.hypotheses[num_return:]
         return results

@@ -10,7 +10,8 @@ hypothesis if it is among the first num_beams, any other becomes a beam until th
 of the best (1 + m) num_beams candidates go on, so that many are asked for.)  A hypothesis of n new tokens scores
 (sum of its tokens' log-probabilities) / n ** length_penalty.  The best num_beams hypotheses are kept.  A request ends when
 num_beams are finished and no beam can still do better (with ``early_stopping``: when num_beams are finished), or at
-``max_new_tokens``, where its beams become hypotheses too.
+``max_new_tokens``, where its beams become hypotheses too, or with what is finished when no continuation has a finite
+log-probability.  A request that has nothing finished then fails: ``NoContinuation``, raised when all others are done.
 
 The loop's decisions need no GPU: it talks to a ``BeamBackend``, which in tests is a fake.
 """
@@ -75,6 +76,15 @@ class BeamResult:
     @property
     def tokens(self) -> List[int]:
         return self.hypotheses[0].tokens
+
+
+class NoContinuation(RuntimeError):
+    """Requests for which no continuation had a finite log-probability before a hypothesis was finished.  ``results``: those of all
+    requests; of these ones without hypotheses."""
+
+    def __init__(self, failed: Sequence[int], results: List[BeamResult]):
+        super().__init__(", ".join(f"request {i}" for i in failed) + ": no continuation has a finite log-probability")
+        self.failed, self.results = list(failed), results
 
 
 class BeamBackend:
@@ -186,6 +196,7 @@ class BeamLoop:
         return n
 
     def run(self, requests: Sequence[BeamRequest]) -> List[BeamResult]:
+        """The requests' results in their order; ``NoContinuation`` has them too."""
         results = [BeamResult(r.request_id) for r in requests]
         waiting = list(enumerate(requests))
         while waiting:
@@ -203,6 +214,9 @@ class BeamLoop:
                 for l in live:                                   # only on an error
                     for s in l.slots:
                         self.backend.release(s)
+        failed = [r.request_id for r in results if not r.hypotheses]
+        if failed:
+            raise NoContinuation(failed, results)
         return results
 
     def _step(self, live: List[_Live], first: bool, results: List[BeamResult]) -> List[_Live]:
@@ -219,8 +233,6 @@ class BeamLoop:
         still, moves = [], []
         for l, lo, hi in zip(live, first_part, first_part[1:]):
             found = [c for part in range(lo, hi) for c in zip(scores[part], rows[part], tokens[part]) if c[1] >= 0]
-            if not found:
-                raise RuntimeError(f"request {l.request.request_id}: no continuation has a finite log-probability")
             if hi - lo > 1:
                 found.sort(key=lambda c: -c[0])                  # stable: the lower rows first where scores tie
             l.take([c[0] for c in found], [beams[c[1]] for c in found], [c[2] for c in found])

@@ -425,3 +425,38 @@ def test_more_stop_tokens_than_a_selection_has_room_for_are_refused():
     BeamRequest([1], 2, 64, stop_token_ids=tuple(range(64)))
     with pytest.raises(ValueError, match="64 beams and 65 stop tokens"):
         BeamRequest([1], 2, 64, stop_token_ids=tuple(range(65)))
+
+
+# ------------------------------------------------------------------------------------------------- nothing to go on with
+class Dies(Table):
+    """After ``when`` tokens a text that begins with 9 has no candidate any more."""
+    when = 3
+
+    def select(self, slots, tokens, scores, start, k):
+        S, R, T = super().select(slots, tokens, scores, start, k)
+        for i, (lo, hi) in enumerate(zip(start[:-1], start[1:])):
+            if hi > lo and self.text[slots[lo]][0] == 9 and len(self.text[slots[lo]]) >= self.when:
+                S[i], R[i], T[i] = [-math.inf] * k, [-1] * k, [-1] * k
+        return S, R, T
+
+
+def test_a_request_without_continuations_does_not_end_the_others():
+    from flashdecode_cuda_b200.engine.beam import NoContinuation
+    lang = Dies(slots=9)
+    reqs = [BeamRequest([1, 2], 4, 3, request_id=5), BeamRequest([9], 4, 2, request_id=6), BeamRequest([3], 6, 3, stop_token_ids=(2,), request_id=7)]
+    with pytest.raises(NoContinuation, match="request 6: no continuation") as e:
+        BeamLoop(lang, 6).run(reqs)
+    results = e.value.results
+    assert e.value.failed == [6] and [r.request_id for r in results] == [5, 6, 7] and results[1].hypotheses == [] and not lang.text
+    for r, q in ((results[0], reqs[0]), (results[2], reqs[2])):
+        assert [h.tokens for h in r.hypotheses] == [t for _, t, _ in by_hand(lang, q.prompt, q.max_new_tokens, q.num_beams, 1.0, q.stop_token_ids)]
+
+
+def test_what_is_finished_stays_where_nothing_goes_on():
+    lang = Dies()
+    lp = lang.logp([9])
+    stop = int(lp.argmax())
+    lang.when = 2                                # the prompt and one more
+    (r,) = BeamLoop(lang).run([BeamRequest([9], 6, 3, stop_token_ids=(stop,))])
+    assert [(h.tokens, h.finish_reason) for h in r.hypotheses] == [([stop], "stop")] and abs(r.hypotheses[0].score - float(lp[stop])) < 1e-12
+    assert not lang.text
