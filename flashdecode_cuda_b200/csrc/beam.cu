@@ -606,7 +606,7 @@ extern "C" int fd_beam_select_set_form(int form) {
 extern "C" int fd_beam_select(const float* logits, int n, int V, const float* scores, const int* start, int R, int k,
                               float* out_s, int* out_row, int* out_tok, void* scratch, int* status, cudaStream_t stream) {
     if (R == 0) return 0;
-    FD_REQUIRE(n > 0 && V > 0 && R > 0, -2, "beam_select: %d rows of %d logits for %d requests", n, V, R);
+    FD_REQUIRE(n >= 0 && V > 0 && R > 0, -2, "beam_select: %d rows of %d logits for %d requests", n, V, R);
     FD_REQUIRE(n <= 65535, -2, "beam_select: %d rows in one call", n);
     FD_REQUIRE(k >= 1 && k <= BM_MAX_K, -2, "beam_select: %d candidates per request; 1 to %d are taken", k, BM_MAX_K);
     FD_REQUIRE(V <= BM_MAX_VOCAB, -2, "beam_select: a vocabulary of %d; up to %d are taken", V, BM_MAX_VOCAB);
@@ -620,7 +620,7 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     // (a request may have all the rows, up to 64)
     const long long smem = 4ll * (n < BM_MAX_ROWS ? n : BM_MAX_ROWS) * ((units + C - 1) / C) * (BM_UNIT / size);
     const bool fits = smem <= 96 * 1024 && R <= 2 * sms;
-    if (fits && g_beam_form != 2 && (g_beam_form == 1 || (n <= BM_CLUSTER_ROWS * R && 4ll * n * V <= BM_CLUSTER_BYTES * R * C))) {
+    if (n > 0 && fits && g_beam_form != 2 && (g_beam_form == 1 || (n <= BM_CLUSTER_ROWS * R && 4ll * n * V <= BM_CLUSTER_BYTES * R * C))) {
         const int which = small ? 2 : (vec ? 1 : 0);
         void (*const kernels[3])(const float*, int, int, const float*, const int*, int, int, int, const BeamOut, int*) = {
             beam_cluster_kernel<false, false>, beam_cluster_kernel<true, false>, beam_cluster_kernel<false, true>};
@@ -639,11 +639,13 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     float* part_m = (float*)(part_s + (size_t)n * p.splits);
     float* gmax = part_m + (size_t)n * p.splits;
     const dim3 grid(p.splits, n);
-    if (small) beam_scan_kernel<false, true><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
-    else if (vec) beam_scan_kernel<true, false><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
-    else beam_scan_kernel<false, false><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
-    int rc = check_launch("beam_select");
-    if (rc != 0) return rc;
+    if (n > 0) {                         // (else requests without rows: the pick says so)
+        if (small) beam_scan_kernel<false, true><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
+        else if (vec) beam_scan_kernel<true, false><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
+        else beam_scan_kernel<false, false><<<grid, BM_SCAN_THREADS, 0, stream>>>(logits, V, units, groups, p.per, gmax, part_m, part_s);
+        const int rc = check_launch("beam_select");
+        if (rc != 0) return rc;
+    }
     return launch_with(true, "beam_select_pick", small ? beam_pick_kernel<BM_SMALL_GROUP> : beam_pick_kernel<BM_GROUP>, dim3(R),
                        dim3(BM_PICK_THREADS), 0, stream, dim3(1, 1, 1), logits, V, n, scores, start, groups, p.splits, (const float*)gmax,
                        (const float*)part_m, (const double*)part_s, k, out, status);

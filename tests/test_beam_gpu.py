@@ -338,3 +338,17 @@ def test_exponentials_of_far_entries():
             assert abs(float(got[0]) - (float(s) - lse)) <= 5 * 2.0 ** -24 * share + 2.0 ** -40, v
     finally:
         K.beam_select_set_form(0)
+
+
+@pytest.mark.parametrize("form", [0, 1, 2])
+@pytest.mark.parametrize("requests", [1, 5, 400])
+def test_requests_without_any_row(form, requests):
+    K.beam_select_set_form(form)
+    try:
+        st = torch.zeros(1, dtype=torch.int32, device=DEV)
+        got = select(torch.zeros(0, 1000), torch.zeros(0), [0] * (requests + 1), 6, status=st)
+        assert bool((got[0] == -math.inf).all()) and bool((got[1] == -1).all()) and bool((got[2] == -1).all()) and int(st.item()) == 0
+        got = select(torch.zeros(0, 1000), torch.zeros(0), [0] * requests + [1], 6, status=st)
+        assert bool((got[1] == -1).all()) and int(st.item()) == K.STATUS_BAD_INDEX
+    finally:
+        K.beam_select_set_form(0)
