@@ -24,6 +24,7 @@
 // 1e-7 are left have no common sign and average out over the row.  Groups of 16 are added in 32 bits, then in 64.
 #include <cooperative_groups.h>
 #include <math.h>
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -610,6 +611,17 @@ extern "C" int fd_beam_select(const float* logits, int n, int V, const float* sc
     FD_REQUIRE(n <= 65535, -2, "beam_select: %d rows in one call", n);
     FD_REQUIRE(k >= 1 && k <= BM_MAX_K, -2, "beam_select: %d candidates per request; 1 to %d are taken", k, BM_MAX_K);
     FD_REQUIRE(V <= BM_MAX_VOCAB, -2, "beam_select: a vocabulary of %d; up to %d are taken", V, BM_MAX_VOCAB);
+    // (places are cleared before the scores are read, and one request's are written while another's rows still are)
+    const auto apart = [](const void* p, long long a, const void* q, long long b) {
+        const unsigned long long x = (unsigned long long)p, y = (unsigned long long)q;
+        return x + a <= y || y + b <= x;
+    };
+    const long long wide = 4ll * R * k;
+    for (const void* o : {(const void*)out_s, (const void*)out_row, (const void*)out_tok})
+        FD_REQUIRE(apart(o, wide, logits, 4ll * n * V) && apart(o, wide, scores, 4ll * n) && apart(o, wide, start, 4ll * (R + 1)), -2,
+                   "beam_select: an output shares memory with an input");
+    FD_REQUIRE(apart(out_s, wide, out_row, wide) && apart(out_s, wide, out_tok, wide) && apart(out_row, wide, out_tok, wide), -2,
+               "beam_select: two outputs share memory");
     const BeamOut out{out_s, out_row, out_tok};
     const bool small = V <= BM_SMALL_VOCAB;
     const bool vec = !small && V % 4 == 0 && (reinterpret_cast<unsigned long long>(logits) & 15) == 0;

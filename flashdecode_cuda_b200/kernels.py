@@ -1677,7 +1677,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, row_start: torch.Ten
     scores[b] + log_softmax(logits[b])[v], best first, the lower row and then the lower token first where they tie, go to
     ``out_scores`` (float32), ``out_rows`` and ``out_tokens`` (int32), all [R, k] with k up to BEAM_MAX_CANDIDATES.  A logit of
     -inf is no candidate; V is at most BEAM_MAX_VOCAB; a row whose score or normaliser is no finite number (a NaN or +inf among its logits, nothing but -inf) has
-    none.  Places that no candidate fills: -inf, -1, -1.  ``scratch``: uint8 of ``beam_select_scratch_bytes(n, V)`` that the call may
+    none.  Places that no candidate fills: -inf, -1, -1.  The outputs share no memory with each other or the
+    inputs.  ``scratch``: uint8 of ``beam_select_scratch_bytes(n, V)`` that the call may
     use; when omitted it is allocated."""
     f32, i32 = torch.float32, torch.int32
     if not (logits.dim() == 2 and logits.dtype is f32 and scores.dtype is f32):

@@ -352,3 +352,20 @@ def test_requests_without_any_row(form, requests):
         assert bool((got[1] == -1).all()) and int(st.item()) == K.STATUS_BAD_INDEX
     finally:
         K.beam_select_set_form(0)
+
+
+def test_outputs_over_inputs_or_each_other_are_refused():
+    """Scores written over the ones that are read would be the natural thing to do with as many candidates as beams."""
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)
+    x, scores, start = torch.randn(4, 100, device=DEV), torch.zeros(4, device=DEV), torch.tensor([0, 2, 4], dtype=torch.int32, device=DEV)
+    both = torch.zeros(12, device=DEV)
+    ints = both.view(torch.int32)
+    for s, out in ((scores, (scores.view(2, 2), i(2, 2), i(2, 2))), (both[:4], (both[2:6].view(2, 2), i(2, 2), i(2, 2))),
+                   (both[3:7], (torch.zeros(2, 2, device=DEV), i(2, 2), ints[:4].view(2, 2))),
+                   (scores, (x[3, 90:94].view(2, 2), i(2, 2), i(2, 2))), (scores, (both[:4].view(2, 2), ints[3:7].view(2, 2), i(2, 2))),
+                   (scores, (both[:4].view(2, 2), ints[4:8].view(2, 2), ints[7:11].view(2, 2)))):
+        with pytest.raises(K.KernelError, match="share"):
+            K.beam_select(x, s, start, *out)
+    K.beam_select(x, both[:4], start, both[4:8].view(2, 2), ints[8:12].view(2, 2), i(2, 2))          # neighbours share nothing
+    want = select(x.cpu(), torch.zeros(4), [0, 2, 4], 2)
+    assert torch.equal(both[4:8].view(2, 2).cpu(), want[0]) and torch.equal(ints[8:12].view(2, 2).cpu(), want[1])
