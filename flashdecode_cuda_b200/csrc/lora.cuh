@@ -96,6 +96,13 @@ __device__ __forceinline__ void lora_copy(const int* tok, int count, const void*
     }
 }
 
+// What rounding to bfloat16 takes away from a sum of A x; nothing from an infinite one (inf - inf would make NaN of every output of its
+// token that the sum reaches, also of those that are infinite).
+__device__ __forceinline__ float lora_rest(float v) {
+    const float h = __bfloat162float(__float2bfloat16_rn(v));
+    return isinf(h) ? 0.f : v - h;
+}
+
 // The most tiles there can be: every segment ends with one that may not be full.
 inline long long lora_max_tiles(const LoraArgs& p, int rows) { return (p.T + (long long)(rows - 1) * p.n_seg) / rows; }
 

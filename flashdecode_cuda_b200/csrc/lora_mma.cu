@@ -341,9 +341,8 @@ lora_rows_kernel(const LoraArgs p, int copies) {
 #pragma unroll 4
             for (int k = 0; k < C; ++k) v += *cluster.map_shared_rank(f, k);
         }
-        const __nv_bfloat16 h = __float2bfloat16_rn(v);
-        hi[row * WB + s * Rc + j] = h;
-        lo[row * WB + s * Rc + j] = __float2bfloat16_rn(v - __bfloat162float(h));
+        hi[row * WB + s * Rc + j] = __float2bfloat16_rn(v);
+        lo[row * WB + s * Rc + j] = __float2bfloat16_rn(lora_rest(v));
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");        // the others' sums have been read
     __syncthreads();

@@ -304,7 +304,9 @@ lora_tile_kernel(const __grid_constant__ LoraMaps maps, const LoraArgs p, const 
                 v[4] += f1.x; v[5] += f1.y; v[6] += f1.z; v[7] += f1.w;
             }
             const uint4 hi = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-            const uint4 lo = make_uint4(pack_bf16_rest(v[0], v[1]), pack_bf16_rest(v[2], v[3]), pack_bf16_rest(v[4], v[5]), pack_bf16_rest(v[6], v[7]));
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = lora_rest(v[q]);
+            const uint4 lo = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
             unsigned char* at = smem + (sl * chunks + j / 64) * LT_TILE + lt_swizzled(row, (j % 64) / 8);
             for (int k = 0; k < C; ++k) {
                 unsigned char* to = cluster.map_shared_rank(at, k);

@@ -448,3 +448,28 @@ def test_more_rows_of_b_than_a_copy_can_name(T, form):
         small = dict(x=x[t:t + 1].cpu(), a=a[e:e + 1].cpu(), b=b[e:e + 1].cpu(), y=y[t:t + 1].cpu(), scale=torch.ones(1))
         want, size, hsize = expected(small, None, 1, [0])
         assert bool(((out[t:t + 1].cpu().double() - want).abs() <= tolerance("bfloat16", small, want, size, hsize)).all())
+
+
+@pytest.mark.parametrize("dtype,form", [("float32", 0), ("bfloat16", 0), ("bfloat16", 1), ("bfloat16", 2)])
+@pytest.mark.parametrize("T", [5, 16, 300])
+def test_an_infinite_sum_gives_what_the_formula_gives(dtype, form, T):
+    """Adapters of rank 1: A x is +inf or -inf for a token with an infinity, and so is every output, with B's sign; NaN where B is zero."""
+    Kd, N, R = 256, 264, 8
+    d, cols, S = make(dtype, T, Kd, N, 2, R, ranks=[1, 1])
+    d["b"][:, 5] = 0.0
+    d["x"][2, 7], d["x"][T - 1, 30] = float("inf"), -float("inf")
+    if form == 0 and dtype == "bfloat16":
+        Kd = 255                                                 # sizes for the CUDA cores
+        d["x"], d["a"] = d["x"][:, :Kd].contiguous(), d["a"][:, :, :Kd].contiguous()
+    token = [i % 2 for i in range(T)]
+    K.lora_set_form(form)
+    try:
+        got = run(d, cols, S, token)
+    finally:
+        K.lora_set_form(0)
+    for t in (2, T - 1):
+        e = token[t]
+        h = (d["a"][e, 0].double() * d["x"][t].double()).sum()
+        want = d["y"][t].double() + float(d["scale"][e]) * d["b"][e, :, 0].double() * h
+        assert bool(h.isinf()) and bool(want[5].isnan()) and int(want.isinf().sum()) == N - 1
+        assert torch.equal(got[t].double().nan_to_num(nan=0.5, posinf=1.0, neginf=-1.0), want.nan_to_num(nan=0.5, posinf=1.0, neginf=-1.0))
