@@ -12,7 +12,7 @@
 // CTA picks from there - one launch, no memory in between.  More: one kernel streams all rows with the whole GPU, a second one picks
 // (the clusters' other CTAs would hold their SMs while the first ones pick).
 //
-// What bounds it.  Many requests: the scan, by HBM.  64 requests of 8 rows of 152,064 (311 MB, floor 47.6 us) take 62.8 us: the scan 52 (6.0
+// What bounds it.  Many requests: the scan, by HBM.  64 requests of 8 rows of 152,064 (311 MB, floor 47.6 us) take 62.9 us: the scan 52 (6.0
 // TB/s), the pick 11 - a chain of a few dozen block-wide steps on 64 CTAs, which starts early (programmatic launch) but has nothing to do
 // before the last row's maxima are there.  Few requests: latency.  One request of 4 rows of 151,936 takes 12 us and seven of 3 to
 // 8 rows of 50,257 13, of which the bytes would be 0.4 and 1.1: launch and cluster start 3, streaming 160 KB per CTA 4, the pick 5.
@@ -580,7 +580,7 @@ using namespace fd;
 
 // Bytes of logits per CTA, and rows per request, up to which the one launch is taken.  Measured, clusters / two kernels, us on the device (a
 // call costs the host 10 to 13 and 12 to 17 us, which is what counts when calls follow each other): 4 rows of 151,936 (152 KB per CTA)
-// 12.1 / 10.4; 36 ragged rows of 50,257 for 7 requests (65 KB) 13.1 / 10.6; 64 rows of 32,000 for 16 10.1 / 9.5; 106 rows of 2,410 for 53
+// 12.1 / 10.4; 36 ragged rows of 50,257 for 7 requests (65 KB) 13.2 / 10.7; 64 rows of 32,000 for 16 10.1 / 9.5; 106 rows of 2,410 for 53
 // 8.2 / 8.4; but 117 of 120,971 for 13 (272 KB) 31 / 22, 512 of 152,064 for 64 93 / 63; 22 rows of 14,151 for one request 21 / 14.5, 240
 // of 1,000 for 8 15.8 / 11.6: many rows have many maxima, and of the two picks the one of 1,024 threads that reads them from L2 is the faster.
 constexpr long long BM_CLUSTER_BYTES = 160 * 1024;

@@ -6,7 +6,7 @@
 // CTA expands its share of the N columns.  A x never leaves the chip and no second launch waits for the first.
 // All sums are 32-bit; one rounding at the end.  The cuts of K depend on the sizes alone, so that no bit of a token's result
 // depends on the other tokens of the step.
-// What bounds it.  A few tokens: latency (24 tokens of 5 adapters, float32, 8960 x 1536, rank 16: 10.6 us; the bytes would take 0.5): launch
+// What bounds it.  A few tokens: latency (24 tokens of 5 adapters, float32, 8960 x 1536, rank 16: 10.5 us; the bytes would take 0.5): launch
 // and cluster start, one trip for the segments and one for the tokens, one pass over a CTA's share of A, the exchange, one pass over B.
 // Many tokens: the FMAs and what they read from shared memory, since every tile of 16 reads its matrices anew (800 tokens, float32, three
 // slices of rank 33, 464 x 5224: 64 us; the bytes would take 7).  bfloat16 comes here only with sizes that are no multiples of 8.

@@ -10,10 +10,10 @@
 //   * the sums of A x are 32-bit.  B h takes h as two bfloat16 numbers (what rounding takes away from the first is the second),
 //     which is 2^-17 of h apart from it and costs one more MMA on operands that are there already.
 //
-// Measured (device time): 48 tokens of 12 adapters, gate and up of 3584 x 37888, rank 64 (54 MB, floor 8.3 us): 24.2 us - finding the tile 1.3,
+// Measured (device time): 48 tokens of 12 adapters, gate and up of 3584 x 37888, rank 64 (54 MB, floor 8.3 us): 24.0 us - finding the tile 1.3,
 // A x 4.5, the exchange 3 to 4, B h 11.7.  The last is what a warp's passes of 32 columns take to come and go (weights, y and the store of
 // each: three trips, the next pass's weights asked for before this one multiplies); DRAM is at 32 % of its rate, the tensor pipe at 6 %.
-// One token, q/k/v of 1536 x 2048, rank 16: 6.2 us, launch and the chain of trips.  2,179 tokens, 611 of them without an adapter, 3584 x 3584, rank 32: 22.5 us
+// One token, q/k/v of 1536 x 2048, rank 16: 6.0 us, launch and the chain of trips.  2,179 tokens, 611 of them without an adapter, 3584 x 3584, rank 32: 21.9 us
 // (floor 6.6), bound by what the tiles read of A and B out of L2.
 #include <cooperative_groups.h>
 

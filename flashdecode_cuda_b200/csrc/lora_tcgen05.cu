@@ -3,8 +3,8 @@
 // Such a step reads x and y and writes out, and does 2 r operations with every element of them, so it is bound by memory as long
 // as the products keep up: at rank 64 they would take all that mma.sync has, which is why they are tcgen05.mma here.  A cluster of CTAs
 // takes 128 tokens of one adapter:
-//   1. D1 [128 x S r] = x A^T over the CTA's share of K, in tensor memory.  Blocks of 64 columns of x and A go through a ring of
-//      swizzled tiles.
+//   1. D1 [128 x S r] = x A^T over the CTA's share of K, in tensor memory: one 32-bit sum over all of it (one output in 240 is a bfloat16
+//      step from that of shorter sums, one in 390 with tiles of 16).  Blocks of 64 columns of x and A go through a ring of swizzled tiles.
 //   2. The cluster's partial sums are added in the order of the ranks: each CTA adds 128 / C tokens' and hands them to all,
 //      as two bfloat16 numbers each (what rounding takes away from the first is the second: 2^-17 of A x is lost, not 2^-9).
 //   3. D2 [128 x 128] = h B^T for the CTA's share of the columns, a product for every slice that has columns in the tile (gate and up
@@ -15,7 +15,7 @@
 // A wait that runs out before step 2 stops the whole cluster: its sums lack a part, and nothing is stored.  One in step 3 stops its own
 // CTA, whose tiles from there on stay as they were.  Copies and MMAs in flight end before their memory is used again or given up.
 //
-// Measured: four prompts of 1,900 to 2,048 tokens, 13824 x 5120, rank 64 (390 MB, floor 59.7 us): 93 us, 4.2 TB/s - finding the tile 3, step 1 47
+// Measured: four prompts of 1,900 to 2,048 tokens, 13824 x 5120, rank 64 (390 MB, floor 59.7 us): 92 us, 4.2 TB/s - finding the tile 3, step 1 47
 // (an SM takes 57 GB/s, a third of it A, which every tile reads anew out of L2), step 2 5, step 3 32 (5.1 TB/s of y and out).  The two
 // streams follow one another, the exchange stands between them, and 65 tiles in clusters of 2 leave 18 SMs idle.  Tensor pipe 11 %.
 #include <cooperative_groups.h>
