@@ -42,12 +42,9 @@ class BeamRequest:
             raise ValueError("max_new_tokens must be >= 1")
         if not (1 <= self.num_beams <= K.BEAM_MAX_ROWS):
             raise ValueError(f"num_beams must lie in 1..{K.BEAM_MAX_ROWS}, got {self.num_beams}")
+        self.stops = len(set(self.stop_token_ids))
         if self.num_beams + self.stops > K.BEAM_MAX_CANDIDATES:
             raise ValueError(f"{self.num_beams} beams and {self.stops} stop tokens; {K.BEAM_MAX_CANDIDATES} in all are taken")
-
-    @property
-    def stops(self) -> int:
-        return len(set(self.stop_token_ids))
 
     def candidates(self, rows: int) -> int:
         """How many of the best candidates of ``rows`` beams hold all that may be taken: each beam has at most ``stops`` that end."""
