@@ -178,22 +178,28 @@ class BeamLoop:
             raise ValueError("max_batch must be >= 1")
         self.backend, self.max_batch = backend, max_batch
 
-    def _start(self, waiting: List[Tuple[int, BeamRequest]]) -> int:
+    def _room(self) -> Tuple[int, int]:
         slots, tokens = self.backend.beam_capacity()
-        slots = min(slots, self.max_batch)
+        return min(slots, self.max_batch), tokens
+
+    def _start(self, waiting: List[Tuple[int, BeamRequest]]) -> int:
+        slots, tokens = self._room()
         n = 0
         for _, r in waiting:
             need = self.backend.beam_tokens_held(r)
-            if n == 0 and (r.num_beams > slots or need > tokens):
-                raise ValueError(f"request {r.request_id}: {r.num_beams} beams of {len(r.prompt)} prompt + {r.max_new_tokens} new tokens "
-                                 f"need {r.num_beams} slots and {need} cache tokens; there are {slots} and {tokens}")
-            if r.num_beams > slots or need > tokens:
+            if r.num_beams > slots or need > tokens:             # (each has room alone)
                 break
             n, slots, tokens = n + 1, slots - r.num_beams, tokens - need
         return n
 
     def run(self, requests: Sequence[BeamRequest]) -> List[BeamResult]:
         """The requests' results in their order; ``NoContinuation`` has them too."""
+        slots, tokens = self._room()
+        for r in requests:                                       # before any of them has run
+            need = self.backend.beam_tokens_held(r)
+            if r.num_beams > slots or need > tokens:
+                raise ValueError(f"request {r.request_id}: {r.num_beams} beams of {len(r.prompt)} prompt + {r.max_new_tokens} new tokens "
+                                 f"need {r.num_beams} slots and {need} cache tokens; there are {slots} and {tokens}")
         results = [BeamResult(r.request_id) for r in requests]
         waiting = list(enumerate(requests))
         while waiting:

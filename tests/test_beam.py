@@ -460,3 +460,11 @@ def test_what_is_finished_stays_where_nothing_goes_on():
     (r,) = BeamLoop(lang).run([BeamRequest([9], 6, 3, stop_token_ids=(stop,))])
     assert [(h.tokens, h.finish_reason) for h in r.hypotheses] == [([stop], "stop")] and abs(r.hypotheses[0].score - float(lp[stop])) < 1e-12
     assert not lang.text
+
+
+def test_a_request_without_room_is_refused_before_others_have_run():
+    lang = Table(slots=4)
+    for bad in (BeamRequest([1], 3, 5, request_id=1), BeamRequest([1] * 5000, 3, 2, request_id=1)):
+        with pytest.raises(ValueError, match="request 1: "):
+            BeamLoop(lang).run([BeamRequest([1], 3, 4), bad])
+    assert lang.calls == 0 and not lang.text
