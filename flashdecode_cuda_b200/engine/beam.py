@@ -178,12 +178,7 @@ class BeamLoop:
             raise ValueError("max_batch must be >= 1")
         self.backend, self.max_batch = backend, max_batch
 
-    def _room(self) -> Tuple[int, int]:
-        slots, tokens = self.backend.beam_capacity()
-        return min(slots, self.max_batch), tokens
-
-    def _start(self, waiting: List[Tuple[int, BeamRequest]]) -> int:
-        slots, tokens = self._room()
+    def _start(self, waiting: List[Tuple[int, BeamRequest]], slots: int, tokens: int) -> int:
         n = 0
         for _, r in waiting:
             need = self.backend.beam_tokens_held(r)
@@ -194,7 +189,8 @@ class BeamLoop:
 
     def run(self, requests: Sequence[BeamRequest]) -> List[BeamResult]:
         """The requests' results in their order; ``NoContinuation`` has them too."""
-        slots, tokens = self._room()
+        slots, tokens = self.backend.beam_capacity()
+        slots = min(slots, self.max_batch)
         for r in requests:                                       # before any of them has run
             need = self.backend.beam_tokens_held(r)
             if r.num_beams > slots or need > tokens:
@@ -203,7 +199,7 @@ class BeamLoop:
         results = [BeamResult(r.request_id) for r in requests]
         waiting = list(enumerate(requests))
         while waiting:
-            n = self._start(waiting)
+            n = self._start(waiting, slots, tokens)
             batch, waiting = waiting[:n], waiting[n:]
             live: List[_Live] = []
             try:

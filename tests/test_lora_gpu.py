@@ -473,3 +473,16 @@ def test_an_infinite_sum_gives_what_the_formula_gives(dtype, form, T):
         want = d["y"][t].double() + float(d["scale"][e]) * d["b"][e, :, 0].double() * h
         assert bool(h.isinf()) and bool(want[5].isnan()) and int(want.isinf().sum()) == N - 1
         assert torch.equal(got[t].double().nan_to_num(nan=0.5, posinf=1.0, neginf=-1.0), want.nan_to_num(nan=0.5, posinf=1.0, neginf=-1.0))
+
+
+@pytest.mark.parametrize("dtype,form", [("float32", 0), ("bfloat16", 1), ("bfloat16", 2)])
+def test_the_same_call_gives_the_same_bits(dtype, form):
+    """Sums over a cluster's CTAs are added in the order of their ranks."""
+    d, cols, S = make(dtype, 700, 4104, 1032, 3, 40)
+    token = [(i // 90) % 3 for i in range(700)]
+    K.lora_set_form(form)
+    try:
+        first = run(d, cols, S, token)
+        assert all(torch.equal(run(d, cols, S, token), first) for _ in range(10))
+    finally:
+        K.lora_set_form(0)
